@@ -153,6 +153,37 @@ int xaxb_gemm_fp8_formats(xaxb_ctx* ctx, void* stream, const void* a_fp8, int64_
                           const float* row_mul, int row_mul_stride, const float* col_mul, int col_mul_stride,
                           const void* bias_bf16, const void* residual_bf16, int64_t ldr, void* out_bf16, int64_t ldo);
 
+/*
+ * Block-scaled e4m3: a tensor is q (e4m3) with float32 multipliers inv_scale, one per block, and stands for
+ * q * inv_scale.  Activations [rows, cols] have a block per row and 128 columns, inv_scale [rows, ceil(cols / 128)];
+ * weights [out, in] one per 128 x 128 square, inv_scale [ceil(out / 128), ceil(in / 128)]; the last block of a row or
+ * column of blocks is cut off at the tensor's edge.  (A finer recipe than the reference's one scale per tensor,
+ * xax/nn/fp8.py:327-336, and the layout in which block-quantised checkpoints store their weights.)
+ *
+ * xaxb_quantize_blocks: amax = max|x| of the block, inv_scale = max(amax / 448, 2^-126), 1 where amax is 0, infinite
+ *   or NaN; q = x / inv_scale rounded to nearest even and clipped to +-448 (NaN stays NaN).  block_rows: 1 or 128.
+ * xaxb_rmsnorm_blocks: the same cast (block_rows 1) of t * rsqrt(mean(t^2) + eps) * weight, t = x + residual, all in
+ *   float32; with residual_bf16 non-NULL sum_bf16 [rows, cols] receives bf16(t) (both or neither).  cols <= 32768.
+ * xaxb_silu_mul_blocks: the same cast (block_rows 1) of gate / (1 + exp(-gate)) * up in float32, gate = gu[:, 0:dim],
+ *   up = gu[:, dim:2*dim] of the [rows, ld] fused gate|up product.
+ * xaxb_gemm_fp8_blocks: out[m, n] = bf16( sum_kb a_inv[m, kb] * b_inv[n / 128, kb] * (sum over block kb of
+ *   a[m, k] * b[n, k]) + bias[n] + residual[m, n] ), sums in float32; a_inv, b_inv contiguous; bias bf16 [N] or NULL,
+ *   residual bf16 [M, ldr] or NULL.
+ *
+ * Tensors are contiguous unless a stride is given and 16-byte aligned; cols, dim, K, lda and ldb are multiples of 16,
+ * N, ld, ldr and ldo of 8.
+ */
+int xaxb_quantize_blocks(xaxb_ctx* ctx, void* stream, const void* x_bf16, int64_t rows, int64_t cols, int block_rows,
+                         void* q_e4m3, float* inv_scale);
+int xaxb_rmsnorm_blocks(xaxb_ctx* ctx, void* stream, const void* x_bf16, const void* residual_bf16,
+                        const void* weight_bf16, float eps, int64_t rows, int64_t cols, void* sum_bf16, void* q_e4m3,
+                        float* inv_scale);
+int xaxb_silu_mul_blocks(xaxb_ctx* ctx, void* stream, const void* gate_up_bf16, int64_t ld, int64_t rows, int64_t dim,
+                         void* q_e4m3, float* inv_scale);
+int xaxb_gemm_fp8_blocks(xaxb_ctx* ctx, void* stream, const void* a_e4m3, int64_t lda, const float* a_inv,
+                         const void* b_e4m3, int64_t ldb, const float* b_inv, int64_t M, int64_t N, int64_t K,
+                         const void* bias_bf16, const void* residual_bf16, int64_t ldr, void* out_bf16, int64_t ldo);
+
 /* Same contract for bf16 operands (lda/ldb in elements): the un-quantised linear /
  * lm_head einsum of xax/arch/attention.py:59-67 (xax/arch/llm.py:213-219). */
 int xaxb_gemm_bf16(xaxb_ctx* ctx, void* stream, const void* a_bf16, int64_t lda, const void* b_bf16, int64_t ldb,

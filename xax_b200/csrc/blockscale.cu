@@ -1,0 +1,295 @@
+// Block-scaled e4m3 casts: one float32 multiplier per 128 columns of a row (activations) or per 128 x 128 square
+// (weights), alone and fused behind RMSNorm (with the residual's addition) and SiLU(gate) * up.
+//
+//   amax = max |v| over the block
+//   inv  = max(amax * (1/448), 2^-126); 1 where amax is 0, infinite or NaN
+//   q    = e4m3(v * (1/inv)), round to nearest even, clipped to +-448; NaN stays NaN
+//
+// so the block stands for q * inv.  Everything between the bf16 inputs and q is float32: one rounding to 8 bits at
+// the end (the floor of 2^-126 keeps 1/inv finite; with it the largest value of a normal block lands on 448).
+//
+// All are bandwidth kernels.  A thread owns 16 consecutive values (two 16-byte loads, one 16-byte store), so the
+// eight threads of a block of 128 are eight neighbouring lanes and its maximum takes three shuffles.
+#include "common.cuh"
+#include "quant_device.cuh"
+
+namespace xaxb {
+
+constexpr int kPiece = 16;               // values per thread and piece
+constexpr int kBlockPieces = 128 / kPiece;
+
+// Magnitudes compare as unsigned bit patterns, which puts NaN above infinity: a NaN in a block reaches its amax.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+__device__ __forceinline__ uint32_t magnitude16(const float (&v)[kPiece]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < kPiece; ++j) m = max(m, magnitude(v[j]));
+  return m;
+}
+
+__device__ __forceinline__ uint32_t lanes8_max(uint32_t m) {
+#pragma unroll
+  for (int o = 1; o < kBlockPieces; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
+
+__device__ __forceinline__ float block_inv_scale(uint32_t amax_bits) {
+  const float inv = fmaxf(__uint_as_float(amax_bits) * (1.0f / 448.0f), 0x1p-126f);
+  return amax_bits == 0 || amax_bits >= 0x7F800000u ? 1.0f : inv;
+}
+
+__device__ __forceinline__ uint4 cast16(const float (&v)[kPiece], float scale) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    w[j] = e4m3x2(v[4 * j] * scale, v[4 * j + 1] * scale) | (e4m3x2(v[4 * j + 2] * scale, v[4 * j + 3] * scale) << 16);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ void load16(const __nv_bfloat16* p, float (&v)[kPiece]) {
+  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+  float lo[8], hi[8];
+  unpack8(a, lo);
+  unpack8(b, hi);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = lo[j], v[8 + j] = hi[j];
+}
+
+__device__ __forceinline__ void zero16(float (&v)[kPiece]) {
+#pragma unroll
+  for (int j = 0; j < kPiece; ++j) v[j] = 0.0f;
+}
+
+// n / d for n < 2^31 by a multiplication with a precomputed reciprocal: with l = ceil(log2 d) and
+// m = floor(2^32 (2^l - d) / d) + 1, n / d = (mulhi(m, n) + n) >> l.
+struct FastDiv {
+  uint32_t d, m, l;
+};
+static FastDiv fast_div(uint32_t d) {
+  uint32_t l = 0;
+  while (l < 32 && (1ull << l) < d) ++l;
+  return {d, (uint32_t)(((1ull << 32) * ((1ull << l) - d)) / d + 1), l};
+}
+__device__ __forceinline__ uint32_t div_by(uint32_t n, const FastDiv f) { return (__umulhi(f.m, n) + n) >> f.l; }
+
+// ---- bf16 rows, a block per 128 columns.  Piece number p = row * pieces_per_row + (columns / 16), rows padded to
+// whole blocks, so inv[p / 8] is the block's place in the row-major [rows, blocks] result for every width.
+__global__ void __launch_bounds__(256) quantize_blocks_kernel(const __nv_bfloat16* __restrict__ x, uint32_t pieces,
+                                                              FastDiv per_row, int cols, uint8_t* __restrict__ q,
+                                                              float* __restrict__ inv) {
+  pdl_trigger();
+  pdl_wait();
+  const uint32_t p = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t row = div_by(p, per_row), col = (p - row * per_row.d) * kPiece;
+  const bool here = p < pieces && col < (uint32_t)cols;
+  const int64_t at = (int64_t)row * cols + col;
+  float v[kPiece];
+  zero16(v);
+  if (here) load16(x + at, v);
+  const float s = block_inv_scale(lanes8_max(magnitude16(v)));
+  if (here) {
+    *reinterpret_cast<uint4*>(q + at) = cast16(v, 1.0f / s);
+    if (p % kBlockPieces == 0) inv[p / kBlockPieces] = s;
+  }
+}
+
+// ---- 128 x 128 squares: one CTA each, four pieces per thread kept in registers across the maximum.
+__global__ void __launch_bounds__(256) quantize_squares_kernel(const __nv_bfloat16* __restrict__ x, int64_t rows, int cols,
+                                                               uint8_t* __restrict__ q, float* __restrict__ inv) {
+  pdl_trigger();
+  pdl_wait();
+  const int64_t row0 = (int64_t)blockIdx.x * 128 + threadIdx.x / kBlockPieces;
+  const int col = blockIdx.y * 128 + (threadIdx.x % kBlockPieces) * kPiece;
+  float v[4][kPiece];
+  uint32_t m = 0;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    zero16(v[u]);
+    if (row0 + u * 32 < rows && col < cols) load16(x + (row0 + u * 32) * cols + col, v[u]);
+    m = max(m, magnitude16(v[u]));
+  }
+  const float s = block_inv_scale(block_max_u32(m));
+  const float r = 1.0f / s;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (row0 + u * 32 < rows && col < cols) *reinterpret_cast<uint4*>(q + (row0 + u * 32) * cols + col) = cast16(v[u], r);
+  if (threadIdx.x == 0) inv[(int64_t)blockIdx.x * gridDim.y + blockIdx.y] = s;
+}
+
+// ---- RMSNorm of x (+ residual): t = x + residual and the norm in float32, one CTA per row, the row in registers.
+template <int NP, int NT>
+__global__ void __launch_bounds__(NT) rmsnorm_blocks_kernel(const __nv_bfloat16* __restrict__ x,
+                                                            const __nv_bfloat16* __restrict__ residual,
+                                                            const __nv_bfloat16* __restrict__ weight, float eps, int cols,
+                                                            int blocks, uint4* __restrict__ sum, uint8_t* __restrict__ q,
+                                                            float* __restrict__ inv) {
+  pdl_trigger();
+  pdl_wait();
+  const int64_t row = blockIdx.x;
+  float v[NP][kPiece];
+  float ss = 0.0f;
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    const int col = (threadIdx.x + k * NT) * kPiece;
+    zero16(v[k]);
+    if (col < cols) {
+      const int64_t at = row * cols + col;
+      load16(x + at, v[k]);
+      if (residual) {
+        float r[kPiece];
+        load16(residual + at, r);
+        float lo[8], hi[8];
+#pragma unroll
+        for (int j = 0; j < kPiece; ++j) {
+          v[k][j] += r[j];
+          (j < 8 ? lo[j & 7] : hi[j & 7]) = v[k][j];
+        }
+        sum[at / 8] = pack8(lo);
+        sum[at / 8 + 1] = pack8(hi);
+      }
+#pragma unroll
+      for (int j = 0; j < kPiece; ++j) ss = fmaf(v[k][j], v[k][j], ss);
+    }
+  }
+  const float n = rsqrtf(block_sum_f32(ss) / (float)cols + eps);
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    const int piece = threadIdx.x + k * NT, col = piece * kPiece;
+    if (col < cols) {
+      float w[kPiece];
+      load16(weight + col, w);
+#pragma unroll
+      for (int j = 0; j < kPiece; ++j) v[k][j] = v[k][j] * n * w[j];
+    }
+    const float s = block_inv_scale(lanes8_max(magnitude16(v[k])));
+    if (col < cols) {
+      *reinterpret_cast<uint4*>(q + row * cols + col) = cast16(v[k], 1.0f / s);
+      if (piece % kBlockPieces == 0) inv[row * blocks + piece / kBlockPieces] = s;
+    }
+  }
+}
+
+// ---- silu(gate) * up, gate and up the two halves of a row of the fused gate | up product.
+__global__ void __launch_bounds__(256) silu_mul_blocks_kernel(const __nv_bfloat16* __restrict__ gate_up, int64_t ld,
+                                                              uint32_t pieces, FastDiv per_row, int dim,
+                                                              uint8_t* __restrict__ q, float* __restrict__ inv) {
+  pdl_trigger();
+  pdl_wait();
+  const uint32_t p = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t row = div_by(p, per_row), col = (p - row * per_row.d) * kPiece;
+  const bool here = p < pieces && col < (uint32_t)dim;
+  float h[kPiece];
+  zero16(h);
+  if (here) {
+    float g[kPiece], u[kPiece];
+    load16(gate_up + row * ld + col, g);
+    load16(gate_up + row * ld + dim + col, u);
+#pragma unroll
+    for (int j = 0; j < kPiece; ++j) h[j] = g[j] / (1.0f + expf(-g[j])) * u[j];
+  }
+  const float s = block_inv_scale(lanes8_max(magnitude16(h)));
+  if (here) {
+    *reinterpret_cast<uint4*>(q + (int64_t)row * dim + col) = cast16(h, 1.0f / s);
+    if (p % kBlockPieces == 0) inv[p / kBlockPieces] = s;
+  }
+}
+
+static bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+
+// What the four casts ask of a [rows, cols] result.
+static int check_rows(const char* what, int64_t rows, int64_t cols) {
+  if (rows <= 0 || cols <= 0 || cols % kPiece != 0) {
+    set_last_error("%s: rows (%lld) must be positive and the width (%lld) a positive multiple of %d", what, (long long)rows,
+                   (long long)cols, kPiece);
+    return XAXB_BAD_ARGUMENT;
+  }
+  if (cols > (1 << 24) || rows > 0x7fffffff || rows * ((cols + 127) / 128) * kBlockPieces > 0x7fffff00ll) {
+    set_last_error("%s: [%lld, %lld] has more than 2^31 pieces of %d values", what, (long long)rows, (long long)cols, kPiece);
+    return XAXB_BAD_ARGUMENT;
+  }
+  return XAXB_OK;
+}
+
+template <int NP, int NT>
+static void launch_rmsnorm_blocks(cudaStream_t s, const void* x, const void* residual, const void* weight, float eps,
+                                  int64_t rows, int cols, void* sum, void* q, float* inv) {
+  launch_kernel(rmsnorm_blocks_kernel<NP, NT>, dim3((unsigned)rows), dim3(NT), 0, s, 1, static_cast<const __nv_bfloat16*>(x),
+                static_cast<const __nv_bfloat16*>(residual), static_cast<const __nv_bfloat16*>(weight), eps, cols,
+                (cols + 127) / 128, static_cast<uint4*>(sum), static_cast<uint8_t*>(q), inv);
+}
+
+}  // namespace xaxb
+
+using namespace xaxb;
+
+extern "C" {
+
+int xaxb_quantize_blocks(xaxb_ctx* ctx, void* stream, const void* x_bf16, int64_t rows, int64_t cols, int block_rows,
+                         void* q_e4m3, float* inv_scale) {
+  if (!ctx || !x_bf16 || !q_e4m3 || !inv_scale || misaligned16(x_bf16) || misaligned16(q_e4m3) ||
+      (block_rows != 1 && block_rows != 128)) {
+    set_last_error("quantize_blocks: x and q must be 16-byte aligned, block_rows 1 or 128");
+    return XAXB_BAD_ARGUMENT;
+  }
+  if (int rc = check_rows("quantize_blocks", rows, cols)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(x_bf16);
+  const int64_t blocks = (cols + 127) / 128;
+  if (block_rows == 128) {
+    if (blocks > 65535) {
+      set_last_error("quantize_blocks: at most 65535 squares side by side");
+      return XAXB_BAD_ARGUMENT;
+    }
+    launch_kernel(quantize_squares_kernel, dim3((unsigned)((rows + 127) / 128), (unsigned)blocks), dim3(256), 0, s, 1, x, rows,
+                  (int)cols, static_cast<uint8_t*>(q_e4m3), inv_scale);
+    return check_launch("quantize_squares_kernel");
+  }
+  const uint32_t per_row = (uint32_t)(blocks * kBlockPieces), pieces = (uint32_t)(rows * per_row);
+  launch_kernel(quantize_blocks_kernel, dim3((pieces + 255) / 256), dim3(256), 0, s, 1, x, pieces, fast_div(per_row), (int)cols,
+                static_cast<uint8_t*>(q_e4m3), inv_scale);
+  return check_launch("quantize_blocks_kernel");
+}
+
+int xaxb_rmsnorm_blocks(xaxb_ctx* ctx, void* stream, const void* x_bf16, const void* residual_bf16, const void* weight_bf16,
+                        float eps, int64_t rows, int64_t cols, void* sum_bf16, void* q_e4m3, float* inv_scale) {
+  if (!ctx || !x_bf16 || !weight_bf16 || !q_e4m3 || !inv_scale || (residual_bf16 != nullptr) != (sum_bf16 != nullptr) ||
+      misaligned16(x_bf16) || misaligned16(residual_bf16) || misaligned16(weight_bf16) || misaligned16(sum_bf16) ||
+      misaligned16(q_e4m3)) {
+    set_last_error("rmsnorm_blocks: tensors must be 16-byte aligned; a sum goes with a residual");
+    return XAXB_BAD_ARGUMENT;
+  }
+  if (int rc = check_rows("rmsnorm_blocks", rows, cols)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int pieces = (int)((cols + 127) / 128) * kBlockPieces;
+#define XAXB_NORM(NP, NT) \
+  launch_rmsnorm_blocks<NP, NT>(s, x_bf16, residual_bf16, weight_bf16, eps, rows, (int)cols, sum_bf16, q_e4m3, inv_scale)
+  if (pieces <= 128) XAXB_NORM(1, 128);
+  else if (pieces <= 256) XAXB_NORM(1, 256);
+  else if (pieces <= 512) XAXB_NORM(1, 512);
+  else if (pieces <= 1024) XAXB_NORM(2, 512);
+  else if (pieces <= 2048) XAXB_NORM(4, 512);
+  else {
+    set_last_error("rmsnorm_blocks: rows of at most 32768 values, got %lld", (long long)cols);
+    return XAXB_UNSUPPORTED;
+  }
+#undef XAXB_NORM
+  return check_launch("rmsnorm_blocks_kernel");
+}
+
+int xaxb_silu_mul_blocks(xaxb_ctx* ctx, void* stream, const void* gate_up_bf16, int64_t ld, int64_t rows, int64_t dim,
+                         void* q_e4m3, float* inv_scale) {
+  if (!ctx || !gate_up_bf16 || !q_e4m3 || !inv_scale || misaligned16(gate_up_bf16) || misaligned16(q_e4m3) || ld % 8 != 0 ||
+      ld < 2 * dim) {
+    set_last_error("silu_mul_blocks: gate_up and q must be 16-byte aligned, ld a multiple of 8 and at least twice the width");
+    return XAXB_BAD_ARGUMENT;
+  }
+  if (int rc = check_rows("silu_mul_blocks", rows, dim)) return rc;
+  const uint32_t per_row = (uint32_t)((dim + 127) / 128 * kBlockPieces), pieces = (uint32_t)(rows * per_row);
+  launch_kernel(silu_mul_blocks_kernel, dim3((pieces + 255) / 256), dim3(256), 0, static_cast<cudaStream_t>(stream), 1,
+                static_cast<const __nv_bfloat16*>(gate_up_bf16), ld, pieces, fast_div(per_row), (int)dim,
+                static_cast<uint8_t*>(q_e4m3), inv_scale);
+  return check_launch("silu_mul_blocks_kernel");
+}
+
+}  // extern "C"

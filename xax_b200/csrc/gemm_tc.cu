@@ -17,13 +17,10 @@
 #include <cstdio>
 #include <cstdlib>
 
-#include "common.cuh"
+#include "gemm_device.cuh"
 
 namespace xaxb {
 
-constexpr int kBM = 128;          // rows of A per tile = UMMA M
-constexpr int kBKBytes = 128;     // K bytes per stage = one swizzle span
-constexpr int kGemmThreads = 192; // 6 warps
 constexpr int kSiteProducer = 1, kSiteMma = 2, kSiteEpilogue = 3, kSiteMmaAcc = 4;
 
 struct GemmParams {
@@ -67,17 +64,6 @@ struct GemmParams {
   float4* ce_part;
   const int32_t* ce_targets;
 };
-
-// Tile order: bands of kBand tile rows, column by column inside a band (row index fastest).  The
-// tiles in flight at any moment then share a few row blocks of A and a few column blocks of B
-// -- a working set that stays in L2 -- instead of sweeping all of A for every column of tiles.
-__device__ __forceinline__ void tile_coords(int kBand, int tile, int tiles_m, int tiles_n, int& tm, int& tn) {
-  const int per_band = kBand * tiles_n;
-  const int band = tile / per_band, r = tile - band * per_band;
-  const int rows = min(kBand, tiles_m - band * kBand);
-  tn = r / rows;
-  tm = band * kBand + (r - tn * rows);
-}
 
 // Default number of K blocks of operand B that a producer asks L2 for ahead of the wait on the
 // previous kernel (GemmParams::prefetch_l2).
@@ -509,39 +495,6 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
 // row slice of the tile over the S CTAs through distributed shared memory (fixed order
 // r = 0..S-1, so results are reproducible), applies the epilogue and stores bf16.  No global
 // scratch, one launch, and each CTA reads only 1/S of A.
-
-__device__ __forceinline__ uint32_t cluster_ctarank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_arrive() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait() {
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-// Address of this CTA's shared-memory location `local_smem_addr` as seen in CTA `cta` of the cluster.
-__device__ __forceinline__ uint32_t dsmem_addr(uint32_t local_smem_addr, uint32_t cta) {
-  uint32_t remote;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local_smem_addr), "r"(cta));
-  return remote;
-}
-
-// Plain (schedulable) distributed-shared-memory load; ordering against the writers comes from
-// the cluster barrier that precedes the reads.
-__device__ __forceinline__ float4 ld_dsmem_f4(uint32_t remote_addr) {
-  float4 v;
-  asm("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-      : "r"(remote_addr));
-  return v;
-}
 
 constexpr int kSiteSkProducer = 5, kSiteSkMma = 6, kSiteSkEpilogue = 7;
 

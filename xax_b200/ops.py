@@ -214,6 +214,129 @@ def dequantize_e5m2(q: torch.Tensor, scale: torch.Tensor, out_dtype=BF16) -> tor
     return out
 
 
+# ---------------------------------------------------------------------------------------
+# block-scaled e4m3: (q, inv_scale) with one float32 multiplier per 128 columns of a row, or per 128 x 128 square
+
+SCALE_BLOCK = 128
+
+
+def _blocks(n: int) -> int:
+    return -(-n // SCALE_BLOCK)
+
+
+def _req_blocks(what: str, t: torch.Tensor, dtype, name: str) -> torch.Tensor:
+    """_req for the block-scaled operators: also 2-D, and on the device whose stream the kernel goes to."""
+    if t.dim() != 2:
+        raise ValueError(f"{what}: {name} must be 2-D, got {tuple(t.shape)}")
+    t = _req(t, dtype, name)
+    _on_current_device(what, t, name)
+    return t
+
+
+def _on_current_device(what: str, t: torch.Tensor, name: str) -> None:
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{what}: {name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _cast_outputs(x: torch.Tensor, rows: int, cols: int, block_rows: int = 1):
+    return (torch.empty((rows, cols), dtype=E4M3, device=x.device),
+            torch.empty((-(-rows // block_rows), _blocks(cols)), dtype=torch.float32, device=x.device))
+
+
+def quantize_blocks(x: torch.Tensor, block_rows: int = 1):
+    """x[rows, cols] bf16 -> (q e4m3 [rows, cols], inv_scale f32 [rows, ceil(cols / 128)]): the cast with one scale per
+    row and 128 columns, or with ``block_rows = 128`` per 128 x 128 square (weights; inv_scale then has
+    ceil(rows / 128) rows).  x ~ q * inv_scale.  cols must be a multiple of 16."""
+    x = _req_blocks("quantize_blocks", x, BF16, "x")
+    if block_rows not in (1, SCALE_BLOCK):
+        raise ValueError(f"quantize_blocks: block_rows must be 1 or {SCALE_BLOCK}, got {block_rows}")
+    rows, cols = x.shape
+    q, inv = _cast_outputs(x, rows, cols, block_rows)
+    if rows == 0:
+        return q, inv
+    ctx, st, lib = _c()
+    check(lib.xaxb_quantize_blocks(ctx, st, ptr(x), rows, cols, block_rows, ptr(q), ptr(inv)), "quantize_blocks")
+    return q, inv
+
+
+def gemm_fp8_blocks(a_q, b_q, a_inv, b_inv, bias=None, residual=None, out=None):
+    """Product of block-scaled operands: activations (a_q e4m3 [M, K], a_inv f32 [M, ceil(K / 128)]) and weights
+    (b_q e4m3 [N, K], b_inv f32 [ceil(N / 128), ceil(K / 128)]) -> bf16 [M, N] = A @ B.T + bias + residual.  K must be
+    a multiple of 16 and N of 8."""
+    what = "gemm_fp8_blocks"
+    if a_q.dtype != E4M3 or b_q.dtype != E4M3 or not a_q.is_cuda or not b_q.is_cuda or a_q.dim() != 2 or b_q.dim() != 2:
+        raise ValueError(f"{what} needs 2-D float8_e4m3fn CUDA operands")
+    (M, K), (N, Kb) = a_q.shape, b_q.shape
+    if K != Kb:
+        raise ValueError(f"{what}: inner dimensions differ ({K} vs {Kb})")
+    if a_q.stride(1) != 1 or b_q.stride(1) != 1:
+        raise ValueError(f"{what}: operands must be K-contiguous")
+    a_inv, b_inv = _req(a_inv, torch.float32, "a_inv"), _req(b_inv, torch.float32, "b_inv")
+    if a_inv.shape != (M, _blocks(K)) or b_inv.shape != (_blocks(N), _blocks(K)):
+        raise ValueError(f"{what}: a_inv {tuple(a_inv.shape)} and b_inv {tuple(b_inv.shape)} must be "
+                         f"({M}, {_blocks(K)}) and ({_blocks(N)}, {_blocks(K)})")
+    if bias is not None:
+        bias = _req(bias, BF16, "bias")
+        if bias.shape != (N,):
+            raise ValueError(f"{what}: bias must be [{N}], got {tuple(bias.shape)}")
+    if out is None:
+        out = torch.empty((M, N), dtype=BF16, device=a_q.device)
+    for name, t in (("residual", residual), ("out", out)):
+        if t is not None and (not t.is_cuda or t.dtype != BF16 or t.shape != (M, N) or (N > 1 and t.stride(1) != 1)):
+            raise ValueError(f"{what}: {name} must be a bfloat16 CUDA tensor [{M}, {N}] with contiguous rows")
+    for name, t in (("a_q", a_q), ("b_q", b_q), ("a_inv", a_inv), ("b_inv", b_inv), ("bias", bias), ("residual", residual),
+                    ("out", out)):
+        if t is not None:
+            _on_current_device(what, t, name)
+    if M == 0:
+        return out
+    ctx, st, lib = _c()
+    check(lib.xaxb_gemm_fp8_blocks(ctx, st, ptr(a_q), a_q.stride(0), ptr(a_inv), ptr(b_q), b_q.stride(0), ptr(b_inv), M, N, K,
+                                   ptr(bias), ptr(residual), 0 if residual is None else residual.stride(0), ptr(out),
+                                   out.stride(0)), what)
+    return out
+
+
+def rmsnorm_blocks(x, weight, eps, *, residual=None):
+    """RMSNorm of x (+ residual) [rows, cols] bf16 followed by the cast of quantize_blocks, in float32 from the inputs to
+    the 8 bits.  Returns (x + residual as bf16, or None without a residual; q; inv_scale)."""
+    what = "rmsnorm_blocks"
+    x = _req_blocks(what, x, BF16, "x")
+    rows, cols = x.shape
+    weight = _req(weight, BF16, "weight")
+    _on_current_device(what, weight, "weight")
+    if weight.shape != (cols,):
+        raise ValueError(f"{what}: weight must be [{cols}], got {tuple(weight.shape)}")
+    total = None
+    if residual is not None:
+        residual = _req_blocks(what, residual, BF16, "residual")
+        if residual.shape != x.shape:
+            raise ValueError(f"{what}: residual {tuple(residual.shape)} must have x's shape {tuple(x.shape)}")
+        total = torch.empty_like(x)
+    q, inv = _cast_outputs(x, rows, cols)
+    if rows == 0:
+        return total, q, inv
+    ctx, st, lib = _c()
+    check(lib.xaxb_rmsnorm_blocks(ctx, st, ptr(x), ptr(residual), ptr(weight), float(eps), rows, cols, ptr(total), ptr(q),
+                                  ptr(inv)), what)
+    return total, q, inv
+
+
+def silu_mul_blocks(gate_up, dim: int):
+    """silu(gate) * up of gate_up [rows, 2*dim] bf16 (gate | up), in float32, followed by the cast of quantize_blocks.
+    Returns (q e4m3 [rows, dim], inv_scale f32 [rows, ceil(dim / 128)])."""
+    gate_up = _req_blocks("silu_mul_blocks", gate_up, BF16, "gate_up")
+    rows, ld = gate_up.shape
+    if dim <= 0 or ld != 2 * dim:
+        raise ValueError(f"silu_mul_blocks: gate_up must be [rows, 2 * {dim}], got {tuple(gate_up.shape)}")
+    q, inv = _cast_outputs(gate_up, rows, dim)
+    if rows == 0:
+        return q, inv
+    ctx, st, lib = _c()
+    check(lib.xaxb_silu_mul_blocks(ctx, st, ptr(gate_up), ld, rows, dim, ptr(q), ptr(inv)), "silu_mul_blocks")
+    return q, inv
+
+
 def lm_head_cross_entropy(hidden, weight, targets, mask=None):
     """Cross-entropy loss and accuracy of hidden bf16 [T, H] against targets int [T] under the head weight bf16
     [V, H], without materialising the [T, V] logits (they are reduced inside the GEMM's epilogue).  ``mask``:
