@@ -111,6 +111,8 @@ class XaxbError(RuntimeError):
 def load() -> ctypes.CDLL:
     """Load (building first if the sources changed and nvcc is present) the shared library."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not _build.is_current():
@@ -135,6 +137,10 @@ def ctx(device: int | None = None) -> c_void_p:
     """The per-device context handle (created on first use)."""
     import torch
 
+    if _ctxs:  # a context exists, so there is a GPU: the path of every call but a device's first
+        h = _ctxs.get(torch.cuda.current_device() if device is None else device)
+        if h is not None:
+            return h
     if not torch.cuda.is_available():
         raise RuntimeError("xax_b200 needs a CUDA device (sm_100a); there is no CPU fallback")
     if device is None:
@@ -151,9 +157,11 @@ def ctx(device: int | None = None) -> c_void_p:
 
 
 def stream_ptr() -> int:
+    """Handle of the current stream of the current device.  (Through the raw getter: building a torch.cuda.Stream object
+    for it takes 3.3 us, as long as a launch.)"""
     import torch
 
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def check(rc: int, what: str) -> None:

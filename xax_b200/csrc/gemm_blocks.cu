@@ -47,6 +47,14 @@ __device__ __forceinline__ float4 ld_dsmem_f4_ordered(uint32_t cluster_addr) {
   return v;
 }
 
+// Barrier over one warpgroup of the pair kernel (two of them promote).
+__device__ __forceinline__ void warpgroup_sync(int which) {
+  if (which == 0)
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+  else
+    asm volatile("bar.sync 2, 128;" ::: "memory");
+}
+
 // bf16(f + bias + residual) of eight neighbouring columns, 16 bytes.
 __device__ __forceinline__ void finish8(const GemmBlocksParams& p, float (&f)[8], int m, int n) {
   if (p.bias) {
@@ -294,6 +302,295 @@ static int launch_decode(const Ctx* ctx, cudaStream_t stream, const GemmBlocksPa
   return check_launch("gemm_blocks_decode_kernel");
 }
 
+// ---------------------------------------------------------------------------------------
+// Many rows: 256 x 256 tiles, each by a pair of CTAs on two SMs (tcgen05.mma.cta_group::2; CTA r of the pair loads rows
+// 128 r .. of both operand tiles and keeps rows 128 r .. of the result).  A K block's product goes to one of two
+// tensor-memory buffers of 256 columns, always freshly written; two warpgroups of promoting threads (thread = row,
+// 128 columns each: one weight square) read it out, scale it and add it to float32 registers while the tensor
+// core fills the other buffer.
+//
+// Per 128-byte K block the tensor core needs 512 cycles, reading the buffer out 256, the packed multiply-adds 128 issue
+// slots: the promotion hides behind the MMAs as long as neither side waits for the other's bookkeeping.  Issuing is what
+// takes time there (a barrier test, an MMA or a commit costs its thread about a hundred cycles), so
+//   * two warps issue, one the even and one the odd K blocks (different buffers, nothing to order between them);
+//   * one barrier opens a K block: full[s] counts both CTAs' copies AND the 16 warps that free the buffer, the latter
+//     arriving on the stage that the block two further on will use;
+//   * one commit closes it, multicast to both CTAs: done[s] frees the stage and hands the product over.
+// Registers: three warpgroups start with 168 each; the issuing one gives up what the promoting ones need.
+constexpr int kPairThreads = 384;
+constexpr int kPairLaunchRegs = 168, kPairPromoteRegs = 216, kPairIssueRegs = 72;
+static_assert(2 * kPairPromoteRegs + kPairIssueRegs <= 3 * kPairLaunchRegs, "register split");
+constexpr int kPairTile = 256;
+constexpr int kPairStages = 5;
+constexpr int kPairOperandBytes = kBM * kBKBytes;          // per CTA, operand and stage
+constexpr int kPairStageBytes = 2 * kPairOperandBytes;
+constexpr int kPairOutBytes = kBM * 128;                   // 128 rows of 64 bf16: one TMA store
+constexpr int kPairSmemBytes = kPairStages * kPairStageBytes + 4 * kPairOutBytes + 256;
+constexpr int kSitePairProducer = 55, kSitePairMma = 56, kSitePairPromote = 57;
+
+__device__ __forceinline__ void umma_commit_both(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(smem_u32(bar)), "h"((uint16_t)3)
+               : "memory");
+}
+
+// (a, b) += (x, y) * s, two float32 in one instruction
+__device__ __forceinline__ void fma2(float& a, float& b, uint32_t x, uint32_t y, float s) {
+  asm("{\n\t.reg .b64 c, v, w;\n\t"
+      "mov.b64 c, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tmov.b64 w, {%4, %4};\n\t"
+      "fma.rn.f32x2 c, v, w, c;\n\t"
+      "mov.b64 {%0, %1}, c;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "r"(x), "r"(y), "f"(s));
+}
+
+__global__ void __launch_bounds__(kPairThreads, 1)
+gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                        const __grid_constant__ CUtensorMap tmap_out, const GemmBlocksParams p, const int tiles_m,
+                        const int tiles_n, const int band) {
+  constexpr uint32_t kIdesc = umma_idesc(kFmtE4M3, kFmtE4M3, 0, 0, 2 * kBM, kPairTile);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* smem_a = smem;
+  uint8_t* smem_b = smem + kPairStages * kPairOperandBytes;
+  uint8_t* smem_out = smem + kPairStages * kPairStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem_out + 4 * kPairOutBytes);  // [kPairStages], the leader's count
+  uint64_t* done = full + kPairStages;                                         // [kPairStages], in each CTA
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + kPairStages);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();  // 0 = leader
+  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  const int num_tiles = tiles_m * tiles_n, nkb = p.num_k_blocks;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) mbar_init(full + s, 2 + 16), mbar_init(done + s, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tmap_a);
+    prefetch_tmap(&tmap_b);
+    prefetch_tmap(&tmap_out);
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers exist before anyone signals across the pair
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_trigger();  // tensor memory is allocated: the next kernel may be scheduled
+  pdl_wait();
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairIssueRegs));
+    if (warp == 8) {
+      // ---------------------------------------------------------------- TMA producer (both CTAs)
+      if (lane == 0) {
+        int stage = 0;
+        long long g = 0;  // K blocks so far, over all tiles
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+          int tm, tn;
+          tile_coords(band, tile, tiles_m, tiles_n, tm, tn);
+          const int m0 = tm * kPairTile + (int)rank * kBM, n0 = tn * kPairTile + (int)rank * kBM;
+          for (int kb = 0; kb < nkb; ++kb, ++g) {
+            if (g >= kPairStages) {
+              ok = mbar_wait(done + stage, phase ^ 1, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSitePairProducer);
+              if (!ok) break;
+            }
+            const uint32_t leader_full = dsmem_addr(smem_u32(full + stage), 0);
+            mbar_arrive_expect_tx_cluster(leader_full, kPairStageBytes);
+            tma_load_2d_pair(smem_a + stage * kPairOperandBytes, &tmap_a, leader_full, kb * kBKBytes, m0);
+            tma_load_2d_pair(smem_b + stage * kPairOperandBytes, &tmap_b, leader_full, kb * kBKBytes, n0);
+            if (++stage == kPairStages) stage = 0, phase ^= 1;
+          }
+        }
+        if (!ok) {  // given up: nothing has moved for the wait limit; a millisecond more for the copies asked for last
+          const unsigned long long t0 = globaltimer_ns();
+          while (globaltimer_ns() - t0 < 1000000ull) {
+          }
+        }
+      }
+    } else if (warp <= 10 && rank == 0) {
+      // ---------------------------------------------------------------- MMA issuers (leader only)
+      if (lane == 0) {
+        const int parity = warp - 9;
+        const uint32_t d_tmem = tmem_base + parity * kPairTile;
+        const long long tiles_here = pair < num_tiles ? (num_tiles - pair + num_pairs - 1) / num_pairs : 0;
+        const long long blocks = tiles_here * nkb;
+        int stage = parity;
+        uint32_t phase = 0;
+        for (long long g = parity; g < blocks; g += 2) {
+          if (!mbar_wait(full + stage, phase, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSitePairMma)) break;
+          tc_fence_after_sync();
+          const uint64_t a_desc = umma_desc_kmajor_sw128(smem_u32(smem_a + stage * kPairOperandBytes));
+          const uint64_t b_desc = umma_desc_kmajor_sw128(smem_u32(smem_b + stage * kPairOperandBytes));
+#pragma unroll
+          for (int k = 0; k < kBKBytes / 32; ++k) umma_pair<true>(d_tmem, a_desc + 2 * k, b_desc + 2 * k, kIdesc, k != 0);
+          umma_commit_both(done + stage);
+          stage += 2;
+          if (stage >= kPairStages) stage -= kPairStages, phase ^= 1;
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ promotion and epilogue (both CTAs)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairPromoteRegs));
+    const int quarter = warp & 3, half = warp >> 2;
+    const int row = quarter * 32 + lane;
+    const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + half * 128;
+    uint8_t* out_blocks = smem_out + half * 2 * kPairOutBytes;
+    int stage = 0, next = 2 % kPairStages;  // the block's stage, and that of the block that will use its buffer next
+    uint32_t phase = 0;
+    int buf = 0;
+    bool ok = true;
+    if (lane == 0) {  // both buffers start free
+      mbar_arrive_cluster(dsmem_addr(smem_u32(full), 0));
+      mbar_arrive_cluster(dsmem_addr(smem_u32(full + 1), 0));
+    }
+    for (int tile = pair; tile < num_tiles; tile += num_pairs) {
+      int tm, tn;
+      tile_coords(band, tile, tiles_m, tiles_n, tm, tn);
+      const int m0 = tm * kPairTile + (int)rank * kBM, m = m0 + row;
+      const int n0 = tn * kPairTile + half * 128;
+      // (rows and columns past the matrix have zero products; they read some multiplier that exists)
+      const float* a_inv = p.a_inv + (long long)min(m, p.M - 1) * nkb;
+      const float* b_inv = p.b_inv + (long long)(min(n0, p.N - 1) / 128) * nkb;
+      float acc[128];
+#pragma unroll
+      for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+      float sa[4], sb[4];  // multipliers of the next four blocks
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sa[j] = j < nkb ? __ldg(a_inv + j) : 0.0f, sb[j] = j < nkb ? __ldg(b_inv + j) : 0.0f;
+      for (int kb0 = 0; kb0 < nkb; kb0 += 4) {
+        float sc[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          sc[j] = sa[j] * sb[j];
+          const int kb = kb0 + 4 + j;
+          sa[j] = kb < nkb ? __ldg(a_inv + kb) : 0.0f;
+          sb[j] = kb < nkb ? __ldg(b_inv + kb) : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (kb0 + j < nkb) {
+            if (ok) ok = mbar_wait(done + stage, phase, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSitePairPromote);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok) {
+              tc_fence_after_sync();
+#pragma unroll
+              for (int c = 0; c < 128; c += 32) {
+                uint32_t r[32];
+                tmem_ld_x32(taddr + buf * kPairTile + c, r);
+                tmem_ld_wait();
+                if (c == 96) {
+                  tc_fence_before_sync();
+                  __syncwarp();
+                  if (lane == 0) mbar_arrive_cluster(dsmem_addr(smem_u32(full + next), 0));
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) fma2(acc[c + i], acc[c + i + 1], r[i], r[i + 1], sc[j]);
+              }
+            }
+            buf ^= 1;
+            if (++stage == kPairStages) stage = 0, phase ^= 1;
+            if (++next == kPairStages) next = 0;
+          }
+        }
+      }
+      // The tile's rows, 128 columns a thread, to two staging blocks and from there by TMA, which clips at M and N.
+      if (quarter == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      warpgroup_sync(half);
+#pragma unroll
+      for (int c = 0; c < 128; c += 8) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = acc[c + i];
+        const int n = n0 + c;
+        if (n < p.N) {
+          float v[8];
+          if (p.bias) {
+            unpack8(__ldg(reinterpret_cast<const uint4*>(p.bias + n)), v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] += v[i];
+          }
+          if (p.residual && m < p.M) {
+            unpack8(*reinterpret_cast<const uint4*>(p.residual + m * p.ldr + n), v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] += v[i];
+          }
+        }
+        *reinterpret_cast<uint4*>(out_blocks + c / 64 * kPairOutBytes + sw128_offset(row, c % 64 / 8)) = pack8(f);
+      }
+      fence_proxy_async_smem();
+      warpgroup_sync(half);
+      if (quarter == 0 && lane == 0 && ok) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          if (n0 + b * 64 < p.N && m0 < p.M)
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+                         ::"l"(&tmap_out), "r"(smem_u32(out_blocks + b * kPairOutBytes)), "r"(n0 + b * 64), "r"(m0)
+                         : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      }
+    }
+    if (quarter == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // no arrival or operand read of the peer can still target a CTA that leaves
+  if (warp == 9) {
+    tc_fence_after_sync();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+  }
+}
+
+// How many CTA pairs can be resident at once (not every SM has a partner).
+static int blocks_resident_pairs(const Ctx* ctx) {
+  static int pairs = 0;
+  if (pairs == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * (ctx->num_sms / 2)));
+    cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = kPairSmemBytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, gemm_blocks_pair_kernel, &cfg);
+    pairs = e == cudaSuccess && n > 0 ? n : ctx->num_sms / 2 - 8;
+  }
+  return pairs;
+}
+
+static int launch_pair(const Ctx* ctx, cudaStream_t stream, const GemmBlocksParams& p) {
+  CUtensorMap ta, tb, tout;
+  if (int rc = make_tmap_2d(ctx, &ta, p.a, 1, (uint64_t)p.K, (uint64_t)p.M, (uint64_t)p.lda, kBKBytes, kBM)) return rc;
+  if (int rc = make_tmap_2d(ctx, &tb, p.b, 1, (uint64_t)p.K, (uint64_t)p.N, (uint64_t)p.ldb, kBKBytes, kBM)) return rc;
+  if (int rc = make_tmap_2d(ctx, &tout, p.out, 2, (uint64_t)p.N, (uint64_t)p.M, (uint64_t)p.ldo * 2, 64, kBM)) return rc;
+  if (int rc = ensure_dynamic_smem<gemm_blocks_pair_kernel>(ctx, kPairSmemBytes, "gemm_blocks_pair_kernel")) return rc;
+  const int tiles_m = (p.M + kPairTile - 1) / kPairTile, tiles_n = (p.N + kPairTile - 1) / kPairTile;
+  const long long tiles = (long long)tiles_m * tiles_n;
+  const int max_pairs = blocks_resident_pairs(ctx);
+  const int pairs = tiles < max_pairs ? (int)tiles : max_pairs;
+  cudaError_t e = launch_kernel(gemm_blocks_pair_kernel, dim3((unsigned)(2 * pairs)), dim3(kPairThreads), kPairSmemBytes, stream,
+                                2u, ta, tb, tout, p, tiles_m, tiles_n, 16);
+  if (e != cudaSuccess) {
+    set_last_error("gemm_blocks_pair_kernel launch: %s", cudaGetErrorString(e));
+    return XAXB_LAUNCH_FAILED;
+  }
+  return check_launch("gemm_blocks_pair_kernel");
+}
+
 }  // namespace xaxb
 
 using namespace xaxb;
@@ -330,6 +627,12 @@ extern "C" int xaxb_gemm_fp8_blocks(xaxb_ctx* ctx_, void* stream, const void* a_
     return XAXB_BAD_ARGUMENT;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const long long pair_tiles = ((M + kPairTile - 1) / kPairTile) * ((N + kPairTile - 1) / kPairTile);
+  if (pair_tiles > 0x3fffffff) {
+    set_last_error("gemm_fp8_blocks: [%lld, %lld] has too many tiles", (long long)M, (long long)N);
+    return XAXB_BAD_ARGUMENT;
+  }
+  if (M > 128 && 2 * pair_tiles >= ctx->num_sms) return launch_pair(ctx, s, p);
   if (M <= 16) return launch_decode<16>(ctx, s, p);
   if (M <= 32) return launch_decode<32>(ctx, s, p);
   if (M <= 64) return launch_decode<64>(ctx, s, p);

@@ -224,23 +224,29 @@ def _blocks(n: int) -> int:
     return -(-n // SCALE_BLOCK)
 
 
-def _req_blocks(what: str, t: torch.Tensor, dtype, name: str) -> torch.Tensor:
-    """_req for the block-scaled operators: also 2-D, and on the device whose stream the kernel goes to."""
-    if t.dim() != 2:
-        raise ValueError(f"{what}: {name} must be 2-D, got {tuple(t.shape)}")
+def _req_blocks(what: str, t: torch.Tensor, dtype, name: str, dim: int = 2) -> torch.Tensor:
+    """_req for the block-scaled operators: also of rank ``dim``, and on the device whose stream the kernel goes to."""
+    if t.dim() != dim:
+        raise ValueError(f"{what}: {name} must be {dim}-D, got {tuple(t.shape)}")
     t = _req(t, dtype, name)
-    _on_current_device(what, t, name)
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{what}: {name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
     return t
 
 
-def _on_current_device(what: str, t: torch.Tensor, name: str) -> None:
-    if t.device.index != torch.cuda.current_device():
+def _req_rows(what: str, t: torch.Tensor, dtype, name: str) -> None:
+    """The same for an operand that is read or written through its row stride, with nothing copied."""
+    if not t.is_cuda or t.dtype != dtype or t.dim() != 2:
+        raise ValueError(f"{what}: {name} must be a 2-D {dtype} CUDA tensor (there is no CPU fallback)")
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        raise ValueError(f"{what}: the rows of {name} must be contiguous")
+    if t.get_device() != torch.cuda.current_device():
         raise ValueError(f"{what}: {name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
 def _cast_outputs(x: torch.Tensor, rows: int, cols: int, block_rows: int = 1):
-    return (torch.empty((rows, cols), dtype=E4M3, device=x.device),
-            torch.empty((-(-rows // block_rows), _blocks(cols)), dtype=torch.float32, device=x.device))
+    return (x.new_empty((rows, cols), dtype=E4M3),
+            x.new_empty((-(-rows // block_rows), -(-cols // SCALE_BLOCK)), dtype=torch.float32))
 
 
 def quantize_blocks(x: torch.Tensor, block_rows: int = 1):
@@ -264,36 +270,38 @@ def gemm_fp8_blocks(a_q, b_q, a_inv, b_inv, bias=None, residual=None, out=None):
     (b_q e4m3 [N, K], b_inv f32 [ceil(N / 128), ceil(K / 128)]) -> bf16 [M, N] = A @ B.T + bias + residual.  K must be
     a multiple of 16 and N of 8."""
     what = "gemm_fp8_blocks"
-    if a_q.dtype != E4M3 or b_q.dtype != E4M3 or not a_q.is_cuda or not b_q.is_cuda or a_q.dim() != 2 or b_q.dim() != 2:
-        raise ValueError(f"{what} needs 2-D float8_e4m3fn CUDA operands")
+    _req_rows(what, a_q, E4M3, "a_q")
+    _req_rows(what, b_q, E4M3, "b_q")
     (M, K), (N, Kb) = a_q.shape, b_q.shape
     if K != Kb:
         raise ValueError(f"{what}: inner dimensions differ ({K} vs {Kb})")
-    if a_q.stride(1) != 1 or b_q.stride(1) != 1:
-        raise ValueError(f"{what}: operands must be K-contiguous")
-    a_inv, b_inv = _req(a_inv, torch.float32, "a_inv"), _req(b_inv, torch.float32, "b_inv")
+    a_inv = _req_blocks(what, a_inv, torch.float32, "a_inv")
+    b_inv = _req_blocks(what, b_inv, torch.float32, "b_inv")
     if a_inv.shape != (M, _blocks(K)) or b_inv.shape != (_blocks(N), _blocks(K)):
         raise ValueError(f"{what}: a_inv {tuple(a_inv.shape)} and b_inv {tuple(b_inv.shape)} must be "
                          f"({M}, {_blocks(K)}) and ({_blocks(N)}, {_blocks(K)})")
     if bias is not None:
-        bias = _req(bias, BF16, "bias")
-        if bias.shape != (N,):
+        bias = _req_blocks(what, bias, BF16, "bias", 1)
+        if bias.shape[0] != N:
             raise ValueError(f"{what}: bias must be [{N}], got {tuple(bias.shape)}")
     if out is None:
-        out = torch.empty((M, N), dtype=BF16, device=a_q.device)
-    for name, t in (("residual", residual), ("out", out)):
-        if t is not None and (not t.is_cuda or t.dtype != BF16 or t.shape != (M, N) or (N > 1 and t.stride(1) != 1)):
-            raise ValueError(f"{what}: {name} must be a bfloat16 CUDA tensor [{M}, {N}] with contiguous rows")
-    for name, t in (("a_q", a_q), ("b_q", b_q), ("a_inv", a_inv), ("b_inv", b_inv), ("bias", bias), ("residual", residual),
-                    ("out", out)):
-        if t is not None:
-            _on_current_device(what, t, name)
+        out = a_q.new_empty((M, N), dtype=BF16)
+    else:
+        _req_rows(what, out, BF16, "out")
+        if out.shape != (M, N):
+            raise ValueError(f"{what}: out must be [{M}, {N}], got {tuple(out.shape)}")
+    ldr = 0
+    if residual is not None:
+        _req_rows(what, residual, BF16, "residual")
+        if residual.shape != (M, N):
+            raise ValueError(f"{what}: residual must be [{M}, {N}], got {tuple(residual.shape)}")
+        ldr = residual.stride(0) if M > 1 else N
     if M == 0:
         return out
+    lda, ldo = (a_q.stride(0), out.stride(0)) if M > 1 else (K, N)  # the stride of a single row may be anything
     ctx, st, lib = _c()
-    check(lib.xaxb_gemm_fp8_blocks(ctx, st, ptr(a_q), a_q.stride(0), ptr(a_inv), ptr(b_q), b_q.stride(0), ptr(b_inv), M, N, K,
-                                   ptr(bias), ptr(residual), 0 if residual is None else residual.stride(0), ptr(out),
-                                   out.stride(0)), what)
+    check(lib.xaxb_gemm_fp8_blocks(ctx, st, ptr(a_q), lda, ptr(a_inv), ptr(b_q), b_q.stride(0), ptr(b_inv), M, N, K, ptr(bias),
+                                   ptr(residual), ldr, ptr(out), ldo), what)
     return out
 
 
@@ -303,9 +311,8 @@ def rmsnorm_blocks(x, weight, eps, *, residual=None):
     what = "rmsnorm_blocks"
     x = _req_blocks(what, x, BF16, "x")
     rows, cols = x.shape
-    weight = _req(weight, BF16, "weight")
-    _on_current_device(what, weight, "weight")
-    if weight.shape != (cols,):
+    weight = _req_blocks(what, weight, BF16, "weight", 1)
+    if weight.shape[0] != cols:
         raise ValueError(f"{what}: weight must be [{cols}], got {tuple(weight.shape)}")
     total = None
     if residual is not None:
