@@ -30,6 +30,16 @@ constexpr int kSiteBlkProducer = 51, kSiteBlkMma = 52, kSiteBlkMmaAcc = 53, kSit
 // Barrier over the 128 promoting threads.
 __device__ __forceinline__ void promote_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
+// mbar_wait for barriers that complete within a microsecond: polls before it turns to the clock and the limit, which
+// lives in global memory (reading it once cost a K block of the pair kernel a thousand cycles).
+__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* d_status,
+                                               int code) {
+#pragma unroll 1
+  for (int i = 0; i < 1000; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait(bar, parity, abort_flag, d_status, code);
+}
+
 // A bounded wait that goes on although the CTA has given up: for copies that must land before the CTA may leave.
 __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity, int* d_status) {
   const unsigned long long t0 = globaltimer_ns(), limit = wait_limit_ns(d_status);
@@ -151,7 +161,7 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
       uint32_t phase = 0;
       for (; i < nkb; ++i) {
         if (i >= kStages &&
-            !mbar_wait(done + stage, phase ^ 1, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSiteBlkProducer))
+            !mbar_wait_soon(done + stage, phase ^ 1, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSiteBlkProducer))
           break;
         mbar_arrive_expect_tx(full + stage, Cfg::kStageBytes);
         tma_load_2d(smem_w + stage * Cfg::kWeightBytes, &tmap_w, full + stage, (kb0 + i) * kBKBytes, n0);
@@ -166,10 +176,10 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
       int stage = 0, buf = 0;
       uint32_t phase = 0, buf_phase = 0;
       for (int i = 0; i < nkb; ++i) {
-        if (i >= kBufs && !mbar_wait(buf_free + buf, buf_phase ^ 1, abort_flag, p.d_status,
+        if (i >= kBufs && !mbar_wait_soon(buf_free + buf, buf_phase ^ 1, abort_flag, p.d_status,
                                      XAXB_DEVICE_TIMEOUT * 1000 + kSiteBlkMmaAcc))
           break;
-        if (!mbar_wait(full + stage, phase, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSiteBlkMma)) break;
+        if (!mbar_wait_soon(full + stage, phase, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSiteBlkMma)) break;
         tc_fence_after_sync();
         const uint64_t w_desc = umma_desc_kmajor_sw128(smem_u32(smem_w + stage * Cfg::kWeightBytes));
         const uint64_t x_desc = umma_desc_kmajor_sw128(smem_u32(smem_x + stage * NT * kBKBytes));
@@ -202,8 +212,9 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
           scales[b * NT + t % NT] = m < p.M ? __ldg(a_inv + b) * __ldg(b_inv + i + b) : 0.0f;
         promote_sync();
       }
-      if (ok) ok = mbar_wait(done + stage, phase, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSiteBlkPromote);
-      ok = __all_sync(0xffffffffu, ok);  // (a warp that gave up still takes part in the barriers above)
+      if (lane == 0 && ok)
+        ok = mbar_wait_soon(done + stage, phase, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSiteBlkPromote);
+      ok = __shfl_sync(0xffffffffu, ok, 0);  // (a warp that gave up still takes part in the barriers above)
       if (ok) {
         tc_fence_after_sync();
         const float* sc = scales + in_chunk * NT;
@@ -334,6 +345,13 @@ __device__ __forceinline__ void umma_commit_both(uint64_t* bar) {
                : "memory");
 }
 
+// A load that stays where it is written (an ordinary one is sunk to its first use, behind a wait on the tensor core).
+__device__ __forceinline__ void ld_ahead(float& v, const float* p, bool there) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q ld.global.nc.f32 %0, [%1];\n\t}"
+               : "+f"(v)
+               : "l"(p), "r"((uint32_t)there));
+}
+
 // (a, b) += (x, y) * s, two float32 in one instruction
 __device__ __forceinline__ void fma2(float& a, float& b, uint32_t x, uint32_t y, float s) {
   asm("{\n\t.reg .b64 c, v, w;\n\t"
@@ -399,7 +417,7 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
           const int m0 = tm * kPairTile + (int)rank * kBM, n0 = tn * kPairTile + (int)rank * kBM;
           for (int kb = 0; kb < nkb; ++kb, ++g) {
             if (g >= kPairStages) {
-              ok = mbar_wait(done + stage, phase ^ 1, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSitePairProducer);
+              ok = mbar_wait_soon(done + stage, phase ^ 1, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSitePairProducer);
               if (!ok) break;
             }
             const uint32_t leader_full = dsmem_addr(smem_u32(full + stage), 0);
@@ -425,7 +443,7 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
         int stage = parity;
         uint32_t phase = 0;
         for (long long g = parity; g < blocks; g += 2) {
-          if (!mbar_wait(full + stage, phase, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSitePairMma)) break;
+          if (!mbar_wait_soon(full + stage, phase, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSitePairMma)) break;
           tc_fence_after_sync();
           const uint64_t a_desc = umma_desc_kmajor_sw128(smem_u32(smem_a + stage * kPairOperandBytes));
           const uint64_t b_desc = umma_desc_kmajor_sw128(smem_u32(smem_b + stage * kPairOperandBytes));
@@ -452,55 +470,61 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
       mbar_arrive_cluster(dsmem_addr(smem_u32(full), 0));
       mbar_arrive_cluster(dsmem_addr(smem_u32(full + 1), 0));
     }
+    // The multipliers of the next K block, of this tile or the one after it, are asked for while a block is added.
+    // (Rows and columns past the matrix have zero products; they read some multiplier that exists.)
+    const float *a_inv = nullptr, *b_inv = nullptr;
+    int next_m0 = 0, next_n0 = 0, next_kb = 0, next_tile = pair;
+    float sa = 0.0f, sb = 0.0f;
+    auto ask = [&]() {
+      if (next_kb == 0 && next_tile < num_tiles) {
+        int tm, tn;
+        tile_coords(band, next_tile, tiles_m, tiles_n, tm, tn);
+        next_m0 = tm * kPairTile + (int)rank * kBM;
+        next_n0 = tn * kPairTile + half * 128;
+        a_inv = p.a_inv + (long long)min(next_m0 + row, p.M - 1) * nkb;
+        b_inv = p.b_inv + (long long)(min(next_n0, p.N - 1) / 128) * nkb;
+      }
+      ld_ahead(sa, a_inv + next_kb, next_tile < num_tiles);
+      ld_ahead(sb, b_inv + next_kb, next_tile < num_tiles);
+      if (++next_kb == nkb) next_kb = 0, next_tile += num_pairs;
+    };
+    const uint32_t leader_full = dsmem_addr(smem_u32(full), 0);
+    ask();
     for (int tile = pair; tile < num_tiles; tile += num_pairs) {
-      int tm, tn;
-      tile_coords(band, tile, tiles_m, tiles_n, tm, tn);
-      const int m0 = tm * kPairTile + (int)rank * kBM, m = m0 + row;
-      const int n0 = tn * kPairTile + half * 128;
-      // (rows and columns past the matrix have zero products; they read some multiplier that exists)
-      const float* a_inv = p.a_inv + (long long)min(m, p.M - 1) * nkb;
-      const float* b_inv = p.b_inv + (long long)(min(n0, p.N - 1) / 128) * nkb;
+      const int tile_m0 = next_m0, tile_n0 = next_n0, m = tile_m0 + row;
       float acc[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
-      float sa[4], sb[4];  // multipliers of the next four blocks
+#pragma unroll 1
+      for (int kb = 0; kb < nkb; ++kb) {
+        const float sc = sa * sb;
+        ask();
+        if (!mbar_try_wait(done + stage, phase) && ok)
+          ok = mbar_wait_soon(done + stage, phase, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSitePairPromote);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) {
+          tc_fence_after_sync();
+          const uint32_t from = taddr + buf * kPairTile;
+          uint32_t r[2][32];
+          tmem_ld_x32(from, r[0]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sa[j] = j < nkb ? __ldg(a_inv + j) : 0.0f, sb[j] = j < nkb ? __ldg(b_inv + j) : 0.0f;
-      for (int kb0 = 0; kb0 < nkb; kb0 += 4) {
-        float sc[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          sc[j] = sa[j] * sb[j];
-          const int kb = kb0 + 4 + j;
-          sa[j] = kb < nkb ? __ldg(a_inv + kb) : 0.0f;
-          sb[j] = kb < nkb ? __ldg(b_inv + kb) : 0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (kb0 + j < nkb) {
-            if (ok) ok = mbar_wait(done + stage, phase, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSitePairPromote);
-            ok = __all_sync(0xffffffffu, ok);
-            if (ok) {
-              tc_fence_after_sync();
-#pragma unroll
-              for (int c = 0; c < 128; c += 32) {
-                uint32_t r[32];
-                tmem_ld_x32(taddr + buf * kPairTile + c, r);
-                tmem_ld_wait();
-                if (c == 96) {
-                  tc_fence_before_sync();
-                  __syncwarp();
-                  if (lane == 0) mbar_arrive_cluster(dsmem_addr(smem_u32(full + next), 0));
-                }
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) fma2(acc[c + i], acc[c + i + 1], r[i], r[i + 1], sc[j]);
-              }
+          for (int c = 0; c < 128; c += 32) {  // the next 32 columns are on their way while these are added
+            uint32_t(&now)[32] = r[c / 32 % 2];
+            tmem_ld_wait();
+            if (c < 96) {
+              tmem_ld_x32(from + c + 32, r[(c / 32 + 1) % 2]);
+            } else {
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster(leader_full + next * 8);
             }
-            buf ^= 1;
-            if (++stage == kPairStages) stage = 0, phase ^= 1;
-            if (++next == kPairStages) next = 0;
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) fma2(acc[c + i], acc[c + i + 1], now[i], now[i + 1], sc);
           }
         }
+        buf ^= 1;
+        if (++stage == kPairStages) stage = 0, phase ^= 1;
+        if (++next == kPairStages) next = 0;
       }
       // The tile's rows, 128 columns a thread, to two staging blocks and from there by TMA, which clips at M and N.
       if (quarter == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -510,7 +534,7 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
         float f[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = acc[c + i];
-        const int n = n0 + c;
+        const int n = tile_n0 + c;
         if (n < p.N) {
           float v[8];
           if (p.bias) {
@@ -531,9 +555,9 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
       if (quarter == 0 && lane == 0 && ok) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-          if (n0 + b * 64 < p.N && m0 < p.M)
+          if (tile_n0 + b * 64 < p.N && tile_m0 < p.M)
             asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
-                         ::"l"(&tmap_out), "r"(smem_u32(out_blocks + b * kPairOutBytes)), "r"(n0 + b * 64), "r"(m0)
+                         ::"l"(&tmap_out), "r"(smem_u32(out_blocks + b * kPairOutBytes)), "r"(tile_n0 + b * 64), "r"(tile_m0)
                          : "memory");
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
