@@ -336,8 +336,10 @@ constexpr int kPairStages = 5;
 constexpr int kPairOperandBytes = kBM * kBKBytes;          // per CTA, operand and stage
 constexpr int kPairStageBytes = 2 * kPairOperandBytes;
 constexpr int kPairOutBytes = kBM * 128;                   // 128 rows of 64 bf16: one TMA store
-constexpr int kPairSmemBytes = kPairStages * kPairStageBytes + 4 * kPairOutBytes + 256;
-constexpr int kSitePairProducer = 55, kSitePairMma = 56, kSitePairPromote = 57;
+constexpr int kPairScaleFloats = 132;                      // per stage: the CTA's 128 row multipliers, 2 square multipliers
+constexpr int kPairSmemBytes = kPairStages * (kPairStageBytes + kPairScaleFloats * 4) + 4 * kPairOutBytes + 128;
+static_assert(kPairSmemBytes <= 227 * 1024, "shared memory of a CTA");
+constexpr int kSitePairProducer = 55, kSitePairMma = 56, kSitePairPromote = 57, kSitePairScales = 58;
 
 __device__ __forceinline__ void umma_commit_both(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
@@ -345,11 +347,18 @@ __device__ __forceinline__ void umma_commit_both(uint64_t* bar) {
                : "memory");
 }
 
-// A load that stays where it is written (an ordinary one is sunk to its first use, behind a wait on the tensor core).
-__device__ __forceinline__ void ld_ahead(float& v, const float* p, bool there) {
-  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %2, 0;\n\t@q ld.global.nc.f32 %0, [%1];\n\t}"
-               : "+f"(v)
-               : "l"(p), "r"((uint32_t)there));
+// Two float32 to two bf16, the first in the low half, in one instruction.
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__device__ __forceinline__ void add8(float* f, const uint4 v) {
+  float w[8];
+  unpack8(v, w);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] += w[j];
 }
 
 // (a, b) += (x, y) * s, two float32 in one instruction
@@ -371,7 +380,8 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
   uint8_t* smem_a = smem;
   uint8_t* smem_b = smem + kPairStages * kPairOperandBytes;
   uint8_t* smem_out = smem + kPairStages * kPairStageBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem_out + 4 * kPairOutBytes);  // [kPairStages], the leader's count
+  float* smem_scale = reinterpret_cast<float*>(smem_out + 4 * kPairOutBytes);  // [kPairStages][kPairScaleFloats]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem_scale + kPairStages * kPairScaleFloats);  // [kPairStages], the leader's
   uint64_t* done = full + kPairStages;                                         // [kPairStages], in each CTA
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + kPairStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -382,7 +392,7 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
   const int num_tiles = tiles_m * tiles_n, nkb = p.num_k_blocks;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kPairStages; ++s) mbar_init(full + s, 2 + 16), mbar_init(done + s, 1);
+    for (int s = 0; s < kPairStages; ++s) mbar_init(full + s, 2 + 16), mbar_init(done + s, 2);
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_tmap(&tmap_a);
@@ -454,6 +464,73 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
           if (stage >= kPairStages) stage -= kPairStages, phase ^= 1;
         }
       }
+    } else if (warp == 11) {
+      // ---------------------------------------------------------------- multipliers (both CTAs)
+      // Lane l brings rows l, l + 32, l + 64, l + 96 of a_inv (and lanes 0 and 1 the squares' multipliers) four K blocks at
+      // a time, the next four on their way while these are handed out.  Block g's place in the ring is free once block
+      // g - 3 is done: its MMAs began after every promoting warp had given back the buffer of block g - 5.
+      float next[4][4], next_b[4], now[4][4], now_b[4];
+      const float *a_inv[4] = {}, *b_inv = nullptr;
+      auto enter_tile = [&](int tile) {
+        int tm, tn;
+        tile_coords(band, tile, tiles_m, tiles_n, tm, tn);
+        const int m0 = tm * kPairTile + (int)rank * kBM + lane, n0 = tn * kPairTile + (lane & 1) * 128;
+        // (rows and columns past the matrix have zero products; they get some multiplier that exists)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a_inv[i] = p.a_inv + (long long)min(m0 + 32 * i, p.M - 1) * nkb;
+        b_inv = p.b_inv + (long long)(min(n0, p.N - 1) / 128) * nkb;
+      };
+      auto ask = [&](int kb) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int at = min(kb + j, nkb - 1);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) next[j][i] = __ldg(a_inv[i] + at);
+          next_b[j] = __ldg(b_inv + at);
+        }
+      };
+      if (pair < num_tiles) {
+        enter_tile(pair);
+        ask(0);
+      }
+      int stage = 0, wait_stage = kPairStages - 3;
+      uint32_t wait_phase = 1;  // of block g - 3; the first three blocks find their places free
+      long long g = 0;
+      bool ok = true;
+      for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+        for (int kb0 = 0; kb0 < nkb && ok; kb0 += 4) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) now[j][i] = next[j][i];
+            now_b[j] = next_b[j];
+          }
+          if (kb0 + 4 < nkb) {
+            ask(kb0 + 4);
+          } else if (tile + num_pairs < num_tiles) {
+            enter_tile(tile + num_pairs);
+            ask(0);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (kb0 + j < nkb) {
+              if (g >= 3 && ok)
+                ok = mbar_wait_soon(done + wait_stage, wait_phase, abort_flag, p.d_status,
+                                    XAXB_DEVICE_TIMEOUT * 1000 + kSitePairScales);
+              ok = __all_sync(0xffffffffu, ok);
+              float* to = smem_scale + stage * kPairScaleFloats;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) to[lane + 32 * i] = now[j][i];
+              if (lane < 2) to[128 + lane] = now_b[j];
+              __syncwarp();
+              if (lane == 0) mbar_arrive(done + stage);
+              ++g;
+              if (++stage == kPairStages) stage = 0;
+              if (++wait_stage == kPairStages) wait_stage = 0, wait_phase ^= 1;
+            }
+          }
+        }
+      }
     }
   } else {
     // ------------------------------------------------------------------ promotion and epilogue (both CTAs)
@@ -470,35 +547,17 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
       mbar_arrive_cluster(dsmem_addr(smem_u32(full), 0));
       mbar_arrive_cluster(dsmem_addr(smem_u32(full + 1), 0));
     }
-    // The multipliers of the next K block, of this tile or the one after it, are asked for while a block is added.
-    // (Rows and columns past the matrix have zero products; they read some multiplier that exists.)
-    const float *a_inv = nullptr, *b_inv = nullptr;
-    int next_m0 = 0, next_n0 = 0, next_kb = 0, next_tile = pair;
-    float sa = 0.0f, sb = 0.0f;
-    auto ask = [&]() {
-      if (next_kb == 0 && next_tile < num_tiles) {
-        int tm, tn;
-        tile_coords(band, next_tile, tiles_m, tiles_n, tm, tn);
-        next_m0 = tm * kPairTile + (int)rank * kBM;
-        next_n0 = tn * kPairTile + half * 128;
-        a_inv = p.a_inv + (long long)min(next_m0 + row, p.M - 1) * nkb;
-        b_inv = p.b_inv + (long long)(min(next_n0, p.N - 1) / 128) * nkb;
-      }
-      ld_ahead(sa, a_inv + next_kb, next_tile < num_tiles);
-      ld_ahead(sb, b_inv + next_kb, next_tile < num_tiles);
-      if (++next_kb == nkb) next_kb = 0, next_tile += num_pairs;
-    };
     const uint32_t leader_full = dsmem_addr(smem_u32(full), 0);
-    ask();
     for (int tile = pair; tile < num_tiles; tile += num_pairs) {
-      const int tile_m0 = next_m0, tile_n0 = next_n0, m = tile_m0 + row;
+      int tm, tn;
+      tile_coords(band, tile, tiles_m, tiles_n, tm, tn);
+      const int m0 = tm * kPairTile + (int)rank * kBM, m = m0 + row;
+      const int n0 = tn * kPairTile + half * 128;
       float acc[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
 #pragma unroll 1
       for (int kb = 0; kb < nkb; ++kb) {
-        const float sc = sa * sb;
-        ask();
         if (!mbar_try_wait(done + stage, phase) && ok)
           ok = mbar_wait_soon(done + stage, phase, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSitePairPromote);
         ok = __all_sync(0xffffffffu, ok);
@@ -507,6 +566,8 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
           const uint32_t from = taddr + buf * kPairTile;
           uint32_t r[2][32];
           tmem_ld_x32(from, r[0]);
+          const float* scale = smem_scale + stage * kPairScaleFloats;
+          const float sc = scale[row] * scale[128 + half];
 #pragma unroll
           for (int c = 0; c < 128; c += 32) {  // the next 32 columns are on their way while these are added
             uint32_t(&now)[32] = r[c / 32 % 2];
@@ -527,37 +588,32 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
         if (++next == kPairStages) next = 0;
       }
       // The tile's rows, 128 columns a thread, to two staging blocks and from there by TMA, which clips at M and N.
+      if (p.bias) {
+#pragma unroll
+        for (int c = 0; c < 128; c += 8)
+          if (n0 + c < p.N) add8(&acc[c], __ldg(reinterpret_cast<const uint4*>(p.bias + n0 + c)));
+      }
+      if (p.residual && m < p.M) {
+        const __nv_bfloat16* residual = p.residual + m * p.ldr + n0;
+#pragma unroll
+        for (int c = 0; c < 128; c += 8)
+          if (n0 + c < p.N) add8(&acc[c], *reinterpret_cast<const uint4*>(residual + c));
+      }
       if (quarter == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       warpgroup_sync(half);
 #pragma unroll
-      for (int c = 0; c < 128; c += 8) {
-        float f[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = acc[c + i];
-        const int n = tile_n0 + c;
-        if (n < p.N) {
-          float v[8];
-          if (p.bias) {
-            unpack8(__ldg(reinterpret_cast<const uint4*>(p.bias + n)), v);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] += v[i];
-          }
-          if (p.residual && m < p.M) {
-            unpack8(*reinterpret_cast<const uint4*>(p.residual + m * p.ldr + n), v);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] += v[i];
-          }
-        }
-        *reinterpret_cast<uint4*>(out_blocks + c / 64 * kPairOutBytes + sw128_offset(row, c % 64 / 8)) = pack8(f);
-      }
+      for (int c = 0; c < 128; c += 8)
+        *reinterpret_cast<uint4*>(out_blocks + c / 64 * kPairOutBytes + sw128_offset(row, c % 64 / 8)) =
+            make_uint4(bf16x2(acc[c], acc[c + 1]), bf16x2(acc[c + 2], acc[c + 3]), bf16x2(acc[c + 4], acc[c + 5]),
+                       bf16x2(acc[c + 6], acc[c + 7]));
       fence_proxy_async_smem();
       warpgroup_sync(half);
       if (quarter == 0 && lane == 0 && ok) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-          if (tile_n0 + b * 64 < p.N && tile_m0 < p.M)
+          if (n0 + b * 64 < p.N && m0 < p.M)
             asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
-                         ::"l"(&tmap_out), "r"(smem_u32(out_blocks + b * kPairOutBytes)), "r"(tile_n0 + b * 64), "r"(tile_m0)
+                         ::"l"(&tmap_out), "r"(smem_u32(out_blocks + b * kPairOutBytes)), "r"(n0 + b * 64), "r"(m0)
                          : "memory");
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
