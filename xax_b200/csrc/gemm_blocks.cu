@@ -329,14 +329,14 @@ static int launch_decode(const Ctx* ctx, cudaStream_t stream, const GemmBlocksPa
 //   * one commit closes it, multicast to both CTAs: done[s] frees the stage and hands the product over.
 // Registers: three warpgroups start with 168 each; the issuing one gives up what the promoting ones need.
 constexpr int kPairThreads = 384;
-constexpr int kPairLaunchRegs = 168, kPairPromoteRegs = 216, kPairIssueRegs = 72;
+constexpr int kPairLaunchRegs = 168, kPairPromoteRegs = 192, kPairIssueRegs = 120;
 static_assert(2 * kPairPromoteRegs + kPairIssueRegs <= 3 * kPairLaunchRegs, "register split");
 constexpr int kPairTile = 256;
 constexpr int kPairStages = 5;
 constexpr int kPairOperandBytes = kBM * kBKBytes;          // per CTA, operand and stage
 constexpr int kPairStageBytes = 2 * kPairOperandBytes;
 constexpr int kPairOutBytes = kBM * 128;                   // 128 rows of 64 bf16: one TMA store
-constexpr int kPairScaleFloats = 132;                      // per stage: the CTA's 128 row multipliers, 2 square multipliers
+constexpr int kPairScaleFloats = 132;                      // per stage: 128 row multipliers, 2 of squares, the tile's corner
 constexpr int kPairSmemBytes = kPairStages * (kPairStageBytes + kPairScaleFloats * 4) + 4 * kPairOutBytes + 128;
 static_assert(kPairSmemBytes <= 227 * 1024, "shared memory of a CTA");
 constexpr int kSitePairProducer = 55, kSitePairMma = 56, kSitePairPromote = 57, kSitePairScales = 58;
@@ -361,9 +361,10 @@ __device__ __forceinline__ void add8(float* f, const uint4 v) {
   for (int j = 0; j < 8; ++j) f[j] += w[j];
 }
 
-// (a, b) += (x, y) * s, two float32 in one instruction
+// (a, b) += (x, y) * s, two float32 in one instruction.  (Volatile, which keeps the additions between the loads they
+// overlap with: left to the compiler they gathered behind the last one.)
 __device__ __forceinline__ void fma2(float& a, float& b, uint32_t x, uint32_t y, float s) {
-  asm("{\n\t.reg .b64 c, v, w;\n\t"
+  asm volatile("{\n\t.reg .b64 c, v, w;\n\t"
       "mov.b64 c, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tmov.b64 w, {%4, %4};\n\t"
       "fma.rn.f32x2 c, v, w, c;\n\t"
       "mov.b64 {%0, %1}, c;\n\t}"
@@ -466,15 +467,17 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
       }
     } else if (warp == 11) {
       // ---------------------------------------------------------------- multipliers (both CTAs)
-      // Lane l brings rows l, l + 32, l + 64, l + 96 of a_inv (and lanes 0 and 1 the squares' multipliers) four K blocks at
-      // a time, the next four on their way while these are handed out.  Block g's place in the ring is free once block
+      // Lane l brings rows l, l + 32, l + 64, l + 96 of a_inv (and lanes 0 and 1 the squares' multipliers) two K blocks at a
+      // time, the next two on their way while these are handed out, and with them the tile's first row and column.  Block g's place in the ring is free once block
       // g - 3 is done: its MMAs began after every promoting warp had given back the buffer of block g - 5.
-      float next[4][4], next_b[4], now[4][4], now_b[4];
+      float next[2][4], next_b[2], now[2][4], now_b[2];
       const float *a_inv[4] = {}, *b_inv = nullptr;
+      int corner = 0, next_corner = 0;  // lane 2: the tile's first row; lane 3: its first column
       auto enter_tile = [&](int tile) {
         int tm, tn;
         tile_coords(band, tile, tiles_m, tiles_n, tm, tn);
         const int m0 = tm * kPairTile + (int)rank * kBM + lane, n0 = tn * kPairTile + (lane & 1) * 128;
+        next_corner = lane == 2 ? m0 - lane : tn * kPairTile;
         // (rows and columns past the matrix have zero products; they get some multiplier that exists)
 #pragma unroll
         for (int i = 0; i < 4; ++i) a_inv[i] = p.a_inv + (long long)min(m0 + 32 * i, p.M - 1) * nkb;
@@ -482,7 +485,7 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
       };
       auto ask = [&](int kb) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 2; ++j) {
           const int at = min(kb + j, nkb - 1);
 #pragma unroll
           for (int i = 0; i < 4; ++i) next[j][i] = __ldg(a_inv[i] + at);
@@ -498,21 +501,22 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
       long long g = 0;
       bool ok = true;
       for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
-        for (int kb0 = 0; kb0 < nkb && ok; kb0 += 4) {
+        for (int kb0 = 0; kb0 < nkb && ok; kb0 += 2) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < 2; ++j) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) now[j][i] = next[j][i];
             now_b[j] = next_b[j];
           }
-          if (kb0 + 4 < nkb) {
-            ask(kb0 + 4);
+          corner = kb0 == 0 ? next_corner : corner;
+          if (kb0 + 2 < nkb) {
+            ask(kb0 + 2);
           } else if (tile + num_pairs < num_tiles) {
             enter_tile(tile + num_pairs);
             ask(0);
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < 2; ++j) {
             if (kb0 + j < nkb) {
               if (g >= 3 && ok)
                 ok = mbar_wait_soon(done + wait_stage, wait_phase, abort_flag, p.d_status,
@@ -521,7 +525,7 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
               float* to = smem_scale + stage * kPairScaleFloats;
 #pragma unroll
               for (int i = 0; i < 4; ++i) to[lane + 32 * i] = now[j][i];
-              if (lane < 2) to[128 + lane] = now_b[j];
+              if (lane < 4) to[128 + lane] = lane < 2 ? now_b[j] : __int_as_float(corner);
               __syncwarp();
               if (lane == 0) mbar_arrive(done + stage);
               ++g;
@@ -549,10 +553,7 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
     }
     const uint32_t leader_full = dsmem_addr(smem_u32(full), 0);
     for (int tile = pair; tile < num_tiles; tile += num_pairs) {
-      int tm, tn;
-      tile_coords(band, tile, tiles_m, tiles_n, tm, tn);
-      const int m0 = tm * kPairTile + (int)rank * kBM, m = m0 + row;
-      const int n0 = tn * kPairTile + half * 128;
+      int m0 = 0, n0 = 0;
       float acc[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
@@ -564,23 +565,31 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
         if (ok) {
           tc_fence_after_sync();
           const uint32_t from = taddr + buf * kPairTile;
-          uint32_t r[2][32];
-          tmem_ld_x32(from, r[0]);
+          // Five readouts, each asked for while the one before is added (a wait covers all that are on their way, so
+          // there is one at a time; 32 + 16 columns are what the registers hold beside the 128 sums).
+          uint32_t r[32], t[16];
+          tmem_ld_x32(from, r);
           const float* scale = smem_scale + stage * kPairScaleFloats;
           const float sc = scale[row] * scale[128 + half];
+          if (kb == nkb - 1) m0 = __float_as_int(scale[130]), n0 = __float_as_int(scale[131]) + half * 128;
 #pragma unroll
-          for (int c = 0; c < 128; c += 32) {  // the next 32 columns are on their way while these are added
-            uint32_t(&now)[32] = r[c / 32 % 2];
+          for (int c = 0; c < 128; c += 48) {
             tmem_ld_wait();
             if (c < 96) {
-              tmem_ld_x32(from + c + 32, r[(c / 32 + 1) % 2]);
+              tmem_ld_x16(from + c + 32, t);
             } else {
               tc_fence_before_sync();
               __syncwarp();
               if (lane == 0) mbar_arrive_cluster(leader_full + next * 8);
             }
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) fma2(acc[c + i], acc[c + i + 1], now[i], now[i + 1], sc);
+            for (int i = 0; i < 32; i += 2) fma2(acc[c + i], acc[c + i + 1], r[i], r[i + 1], sc);
+            if (c < 96) {
+              tmem_ld_wait();
+              tmem_ld_x32(from + c + 48, r);
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) fma2(acc[c + 32 + i], acc[c + 33 + i], t[i], t[i + 1], sc);
+            }
           }
         }
         buf ^= 1;
@@ -593,13 +602,13 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
         for (int c = 0; c < 128; c += 8)
           if (n0 + c < p.N) add8(&acc[c], __ldg(reinterpret_cast<const uint4*>(p.bias + n0 + c)));
       }
-      if (p.residual && m < p.M) {
-        const __nv_bfloat16* residual = p.residual + m * p.ldr + n0;
+      if (p.residual && m0 + row < p.M) {
+        const __nv_bfloat16* residual = p.residual + (m0 + row) * p.ldr + n0;
 #pragma unroll
         for (int c = 0; c < 128; c += 8)
           if (n0 + c < p.N) add8(&acc[c], *reinterpret_cast<const uint4*>(residual + c));
       }
-      if (quarter == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      if (quarter < 2 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       warpgroup_sync(half);
 #pragma unroll
       for (int c = 0; c < 128; c += 8)
@@ -608,17 +617,16 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                        bf16x2(acc[c + 6], acc[c + 7]));
       fence_proxy_async_smem();
       warpgroup_sync(half);
-      if (quarter == 0 && lane == 0 && ok) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-          if (n0 + b * 64 < p.N && m0 < p.M)
-            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
-                         ::"l"(&tmap_out), "r"(smem_u32(out_blocks + b * kPairOutBytes)), "r"(n0 + b * 64), "r"(m0)
-                         : "memory");
+      if (quarter < 2 && lane == 0 && ok) {  // a block each
+        const int n = n0 + quarter * 64;
+        if (n < p.N && m0 < p.M)
+          asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+                       ::"l"(&tmap_out), "r"(smem_u32(out_blocks + quarter * kPairOutBytes)), "r"(n), "r"(m0)
+                       : "memory");
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
     }
-    if (quarter == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (quarter < 2 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
   tc_fence_before_sync();
