@@ -82,6 +82,17 @@ __device__ __forceinline__ void finish8(const GemmBlocksParams& p, float (&f)[8]
   *reinterpret_cast<uint4*>(p.out + m * p.ldo + n) = pack8(f);
 }
 
+// (a, b) += (x * s, y * t), two float32 in one instruction.  (Volatile, which keeps the additions between the loads they
+// overlap with: left to the compiler they gathered behind the last one.)
+__device__ __forceinline__ void fma2(float& a, float& b, uint32_t x, uint32_t y, float s, float t) {
+  asm volatile("{\n\t.reg .b64 c, v, w;\n\t"
+               "mov.b64 c, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tmov.b64 w, {%4, %5};\n\t"
+               "fma.rn.f32x2 c, v, w, c;\n\t"
+               "mov.b64 {%0, %1}, c;\n\t}"
+               : "+f"(a), "+f"(b)
+               : "r"(x), "r"(y), "f"(s), "f"(t));
+}
+
 // ---------------------------------------------------------------------------------------
 // Few rows: weight streaming.  The weights are the MMA's 128-row operand and NT rows of activations its columns, so a
 // decode step moves 16 KB of weights and only NT * 128 bytes of activations per K block.  A cluster of S CTAs shares
@@ -93,13 +104,14 @@ __device__ __forceinline__ void finish8(const GemmBlocksParams& p, float (&f)[8]
 //   warps 2-5  promotion: thread = weight row; acc[t] += partial[t] * (a_inv[t, kb] * b_inv[kb]) in float32 registers
 template <int NT>
 struct BlocksDecodeCfg {
-  static constexpr int kCtasPerSm = NT == 128 ? 2 : 3;
+  static constexpr int kCtasPerSm = NT == 16 ? 4 : NT == 32 ? 3 : 2;
   static constexpr int kWeightBytes = kBM * kBKBytes;
   static constexpr int kStageBytes = kWeightBytes + NT * kBKBytes;
-  static constexpr int kStages = NT == 16 ? 4 : 3;
-  static constexpr int kBufs = NT == 16 ? 4 : 2;           // tensor-memory buffers of NT columns
-  static constexpr int kTmemCols = kBufs * NT;              // kCtasPerSm times this is at most 512
-  static constexpr int kScaleBlocks = NT <= 32 ? 32 : 16;  // K blocks whose multipliers are staged at a time
+  static constexpr int kStages = NT == 64 ? 4 : 3;
+  static constexpr int kBufs = 2;                          // tensor-memory buffers of NT columns
+  static constexpr int kTmemCols = kBufs * NT;             // kCtasPerSm times this is at most 512
+  static constexpr int kScaleBlocks = 16;                  // K blocks whose multipliers are staged at a time
+  static constexpr int kLoad = NT == 16 || NT == 128 ? 16 : 32;  // columns per readout (what the registers allow)
   static constexpr int kPipeBytes = kStages * kStageBytes;
   static constexpr int kParkFloats = kBM + 4;              // floats per token of the parked result
   static constexpr int kSmemBytes = kPipeBytes + kScaleBlocks * NT * 4 + 256;
@@ -212,29 +224,31 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
           scales[b * NT + t % NT] = m < p.M ? __ldg(a_inv + b) * __ldg(b_inv + i + b) : 0.0f;
         promote_sync();
       }
-      if (lane == 0 && ok)
+      if (!mbar_try_wait(done + stage, phase) && ok)
         ok = mbar_wait_soon(done + stage, phase, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSiteBlkPromote);
-      ok = __shfl_sync(0xffffffffu, ok, 0);  // (a warp that gave up still takes part in the barriers above)
+      ok = __all_sync(0xffffffffu, ok);  // (a warp that gave up still takes part in the barriers above)
       if (ok) {
         tc_fence_after_sync();
         const float* sc = scales + in_chunk * NT;
+        const uint32_t from = taddr + buf * NT;
 #pragma unroll
-        for (int c = 0; c < NT; c += 16) {
-          uint32_t r[16];
-          tmem_ld_x16(taddr + buf * NT + c, r);
+        for (int c = 0; c < NT; c += Cfg::kLoad) {
+          uint32_t r[Cfg::kLoad];
+          if constexpr (Cfg::kLoad == 32)
+            tmem_ld_x32(from + c, r);
+          else
+            tmem_ld_x16(from + c, r);
           tmem_ld_wait();
-          if (c + 16 == NT) {
+          if (c + Cfg::kLoad == NT) {
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(buf_free + buf);
           }
 #pragma unroll
-          for (int j = 0; j < 16; j += 4) {
+          for (int j = 0; j < Cfg::kLoad; j += 4) {
             const float4 s4 = *reinterpret_cast<const float4*>(sc + c + j);
-            acc[c + j] = fmaf(__uint_as_float(r[j]), s4.x, acc[c + j]);
-            acc[c + j + 1] = fmaf(__uint_as_float(r[j + 1]), s4.y, acc[c + j + 1]);
-            acc[c + j + 2] = fmaf(__uint_as_float(r[j + 2]), s4.z, acc[c + j + 2]);
-            acc[c + j + 3] = fmaf(__uint_as_float(r[j + 3]), s4.w, acc[c + j + 3]);
+            fma2(acc[c + j], acc[c + j + 1], r[j], r[j + 1], s4.x, s4.y);
+            fma2(acc[c + j + 2], acc[c + j + 3], r[j + 2], r[j + 3], s4.z, s4.w);
           }
         }
       }
@@ -359,17 +373,6 @@ __device__ __forceinline__ void add8(float* f, const uint4 v) {
   unpack8(v, w);
 #pragma unroll
   for (int j = 0; j < 8; ++j) f[j] += w[j];
-}
-
-// (a, b) += (x, y) * s, two float32 in one instruction.  (Volatile, which keeps the additions between the loads they
-// overlap with: left to the compiler they gathered behind the last one.)
-__device__ __forceinline__ void fma2(float& a, float& b, uint32_t x, uint32_t y, float s) {
-  asm volatile("{\n\t.reg .b64 c, v, w;\n\t"
-      "mov.b64 c, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tmov.b64 w, {%4, %4};\n\t"
-      "fma.rn.f32x2 c, v, w, c;\n\t"
-      "mov.b64 {%0, %1}, c;\n\t}"
-      : "+f"(a), "+f"(b)
-      : "r"(x), "r"(y), "f"(s));
 }
 
 __global__ void __launch_bounds__(kPairThreads, 1)
@@ -583,12 +586,12 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
               if (lane == 0) mbar_arrive_cluster(leader_full + next * 8);
             }
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) fma2(acc[c + i], acc[c + i + 1], r[i], r[i + 1], sc);
+            for (int i = 0; i < 32; i += 2) fma2(acc[c + i], acc[c + i + 1], r[i], r[i + 1], sc, sc);
             if (c < 96) {
               tmem_ld_wait();
               tmem_ld_x32(from + c + 48, r);
 #pragma unroll
-              for (int i = 0; i < 16; i += 2) fma2(acc[c + 32 + i], acc[c + 33 + i], t[i], t[i + 1], sc);
+              for (int i = 0; i < 16; i += 2) fma2(acc[c + 32 + i], acc[c + 33 + i], t[i], t[i + 1], sc, sc);
             }
           }
         }
