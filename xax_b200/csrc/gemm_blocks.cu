@@ -25,10 +25,13 @@ struct GemmBlocksParams {
   int* d_status;
 };
 
-constexpr int kSiteBlkProducer = 51, kSiteBlkMma = 52, kSiteBlkMmaAcc = 53, kSiteBlkPromote = 54;
+constexpr int kSiteBlkProducer = 51, kSiteBlkMma = 52, kSiteBlkPromote = 53;
 
-// Barrier over the 128 promoting threads.
-__device__ __forceinline__ void promote_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// Barrier over the decode kernel's promoting threads.
+template <int kThreads>
+__device__ __forceinline__ void promote_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+}
 
 // mbar_wait for barriers that complete within a microsecond: polls before it turns to the clock and the limit, which
 // lives in global memory (reading it once cost a K block of the pair kernel a thousand cycles).
@@ -40,10 +43,10 @@ __device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, v
   return mbar_wait(bar, parity, abort_flag, d_status, code);
 }
 
-// A bounded wait that goes on although the CTA has given up: for copies that must land before the CTA may leave.
-__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity, int* d_status) {
-  const unsigned long long t0 = globaltimer_ns(), limit = wait_limit_ns(d_status);
-  while (!mbar_try_wait(bar, parity) && globaltimer_ns() - t0 < limit) {
+// For a producer that has given up: nothing has moved for the wait limit; a millisecond more for the copies asked for last.
+__device__ __forceinline__ void wait_for_last_copies() {
+  const unsigned long long t0 = globaltimer_ns();
+  while (globaltimer_ns() - t0 < 1000000ull) {
   }
 }
 
@@ -98,47 +101,68 @@ __device__ __forceinline__ void fma2(float& a, float& b, uint32_t x, uint32_t y,
 // decode step moves 16 KB of weights and only NT * 128 bytes of activations per K block.  A cluster of S CTAs shares
 // the K blocks of one tile; each CTA leaves its part of the result in shared memory and the cluster adds the parts
 // over distributed shared memory in rank order (no atomics: the same bits every time).
-//   warp 0     TMA producer (weight and activation tiles into a ring)
-//   warp 1     one thread issues the four MMAs of a K block into the next tensor-memory buffer; their commit both
-//              frees the ring stage and hands the block to the promoting warps
-//   warps 2-5  promotion: thread = weight row; acc[t] += partial[t] * (a_inv[t, kb] * b_inv[kb]) in float32 registers
+//   promoting warps  thread = weight row; acc[t] += partial[t] * (a_inv[t, kb] * b_inv[kb]) in float32 registers, up to
+//                    64 tokens a thread (two warpgroups for NT = 128)
+//   next warp        TMA producer (weight and activation tiles into a ring)
+//   next two warps   one thread each issues the four MMAs of every other K block into the next tensor-memory buffer (one
+//                    thread those of all blocks where the ring is too short for two, see issue_step)
+// Finding a barrier complete, an MMA and a commit cost the issuing thread 65 to 200 cycles each, which is what a chain of K
+// blocks runs at, so one barrier opens a block (full[s] counts its copies and the promoting warps that free its buffer,
+// arriving on the stage that the block will use) and one closes it (the commit on done[s] frees the stage and hands the
+// product over).
+// What bounds it is the operand bytes that an SM keeps in flight, so the ring takes all the shared memory that the CTAs
+// which will be resident together leave (`stages`, from the launcher).
 template <int NT>
 struct BlocksDecodeCfg {
-  static constexpr int kCtasPerSm = NT == 16 ? 4 : NT == 32 ? 3 : 2;
+  static constexpr int kGroups = NT == 128 ? 2 : 1;        // promoting warpgroups
+  static constexpr int kCols = NT / kGroups;               // tokens per promoting thread
+  static constexpr int kThreads = NT == 128 ? 384 : 224;
+  // Registers of NT = 128: two CTAs of 384 threads start with 80 a thread; the warpgroup of the producer and the
+  // issuer gives up what the promoting ones need.
+  static constexpr bool kMoveRegs = NT == 128;
+  static constexpr int kPromoteRegs = 104, kIssueRegs = 32;
+  static_assert(kGroups * kPromoteRegs + kIssueRegs <= 3 * 80, "register split");
+  static constexpr int kCtasPerSm = NT <= 32 ? 3 : 2;      // at most: registers, tensor memory
   static constexpr int kWeightBytes = kBM * kBKBytes;
   static constexpr int kStageBytes = kWeightBytes + NT * kBKBytes;
-  static constexpr int kStages = NT == 64 ? 4 : 3;
-  static constexpr int kBufs = 2;                          // tensor-memory buffers of NT columns
-  static constexpr int kTmemCols = kBufs * NT;             // kCtasPerSm times this is at most 512
+  static constexpr int kMaxStages = 12;
+  static constexpr int kBufs = NT == 32 ? 3 : NT == 128 ? 2 : 4;  // tensor-memory buffers of NT columns
+  static constexpr int kTmemCols = NT == 32 ? 128 : kBufs * NT;
   static constexpr int kScaleBlocks = 16;                  // K blocks whose multipliers are staged at a time
   static constexpr int kLoad = NT == 16 || NT == 128 ? 16 : 32;  // columns per readout (what the registers allow)
-  static constexpr int kPipeBytes = kStages * kStageBytes;
   static constexpr int kParkFloats = kBM + 4;              // floats per token of the parked result
-  static constexpr int kSmemBytes = kPipeBytes + kScaleBlocks * NT * 4 + 256;
-  static_assert(NT * kParkFloats * 4 <= kPipeBytes, "the parked result overlays the ring");
-  // A stage's commit barrier must not complete a second time before the promoting warps have seen the first: the
-  // block that uses the stage next has to wait for a buffer that they free after that.
-  static_assert(kBufs <= kStages, "a stage comes round no sooner than a buffer");
-  static_assert(kCtasPerSm * kTmemCols <= 512 && (kCtasPerSm + 1) * (kSmemBytes + 1024) > 228 * 1024,
-                "shared memory must keep more CTAs off the SM than tensor memory serves");
+  static constexpr int kExtraBytes = kScaleBlocks * NT * 4 + (2 * kMaxStages + 1) * 8;
+  static constexpr int kSmemPerSm = 228 * 1024, kSmemReserved = 1024;
+  // The ring that leaves room for `ctas` CTAs on an SM, and for no more of them than tensor memory serves.
+  static constexpr int stages_for(int ctas) {
+    const int n = (kSmemPerSm / ctas - kSmemReserved - kExtraBytes) / kStageBytes;
+    return n < kMaxStages ? n : kMaxStages;
+  }
+  // Two threads may issue if neither can test a stage's barrier a phase early.  A thread that turns to block i has found
+  // block i - 2 open, so the blocks up to i - 2 - kBufs are done; the stage's block before, i - stages, is among them, or
+  // is the same thread's (stages even).
+  static constexpr int issue_step(int stages) { return stages % 2 == 0 || stages >= kBufs + 2 ? 2 : 1; }
+  static constexpr int smem_bytes(int stages) { return stages * kStageBytes + kExtraBytes; }
+  static_assert(NT * kParkFloats * 4 <= 3 * kStageBytes, "the parked result overlays the ring");
+  static_assert(stages_for(kCtasPerSm) >= kBufs && stages_for(kCtasPerSm) >= 3, "a stage comes round no sooner than a buffer");
+  static_assert(kCtasPerSm * kTmemCols <= 512, "tensor memory");
 };
 
 template <int NT>
-__global__ void __launch_bounds__(kGemmThreads, BlocksDecodeCfg<NT>::kCtasPerSm)
+__global__ void __launch_bounds__(BlocksDecodeCfg<NT>::kThreads, BlocksDecodeCfg<NT>::kCtasPerSm)
 gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
-                          const GemmBlocksParams p, const int S) {
+                          const GemmBlocksParams p, const int S, const int stages) {
   using Cfg = BlocksDecodeCfg<NT>;
-  constexpr int kStages = Cfg::kStages, kBufs = Cfg::kBufs;
+  constexpr int kBufs = Cfg::kBufs, kPromoteWarps = 4 * Cfg::kGroups;
   constexpr uint32_t kIdesc = umma_idesc(kFmtE4M3, kFmtE4M3, 0, 0, kBM, NT);
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* smem_w = smem;
-  uint8_t* smem_x = smem + kStages * Cfg::kWeightBytes;
-  float* scales = reinterpret_cast<float*>(smem + Cfg::kPipeBytes);  // [kScaleBlocks][NT]
-  float* park = reinterpret_cast<float*>(smem);                      // [NT][kParkFloats], after the main loop
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kPipeBytes + Cfg::kScaleBlocks * NT * 4);  // [kStages]
-  uint64_t* done = full + kStages;                                   // [kStages]
-  uint64_t* buf_free = done + kStages;                               // [kBufs]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(buf_free + kBufs);
+  uint8_t* smem_x = smem + stages * Cfg::kWeightBytes;
+  float* scales = reinterpret_cast<float*>(smem + stages * Cfg::kStageBytes);  // [kScaleBlocks][NT]
+  float* park = reinterpret_cast<float*>(smem);                                // [NT][kParkFloats], after the main loop
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + Cfg::kScaleBlocks * NT);  // [stages]
+  uint64_t* done = full + Cfg::kMaxStages;                                     // [stages]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + Cfg::kMaxStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -149,14 +173,13 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
   const int nkb = (int)((long long)p.num_k_blocks * (rank + 1) / S) - kb0;  // at least 1: S <= num_k_blocks
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(full + s, 1), mbar_init(done + s, 1);
-    for (int b = 0; b < kBufs; ++b) mbar_init(buf_free + b, 4);
+    for (int s = 0; s < stages; ++s) mbar_init(full + s, 1 + kPromoteWarps), mbar_init(done + s, 1);
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_tmap(&tmap_w);
     prefetch_tmap(&tmap_x);
   }
-  if (warp == 2) {
+  if (warp == kPromoteWarps + 1) {
     tmem_alloc(tmem_slot, Cfg::kTmemCols);
     tmem_relinquish();
   }
@@ -167,30 +190,28 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
   pdl_trigger();  // tensor memory is allocated: the next kernel may be scheduled
   pdl_wait();
 
-  if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0, i = 0;
+  if (warp >= kPromoteWarps) {
+    if constexpr (Cfg::kMoveRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kIssueRegs));
+    if (warp == kPromoteWarps && lane == 0) {
+      // ------------------------------------------------------------------ TMA producer
+      int stage = 0;
       uint32_t phase = 0;
-      for (; i < nkb; ++i) {
-        if (i >= kStages &&
+      for (int i = 0; i < nkb; ++i) {
+        if (i >= stages &&
             !mbar_wait_soon(done + stage, phase ^ 1, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSiteBlkProducer))
           break;
         mbar_arrive_expect_tx(full + stage, Cfg::kStageBytes);
         tma_load_2d(smem_w + stage * Cfg::kWeightBytes, &tmap_w, full + stage, (kb0 + i) * kBKBytes, n0);
         tma_load_2d(smem_x + stage * NT * kBKBytes, &tmap_x, full + stage, (kb0 + i) * kBKBytes, m0);
-        if (++stage == kStages) stage = 0, phase ^= 1;
+        if (++stage == stages) stage = 0, phase ^= 1;
       }
-      if (*abort_flag)  // the stages in flight land before the CTA leaves
-        for (int j = i > kStages ? i - kStages : 0; j < i; ++j) mbar_drain(full + j % kStages, (j / kStages) & 1, p.d_status);
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0, buf = 0;
-      uint32_t phase = 0, buf_phase = 0;
-      for (int i = 0; i < nkb; ++i) {
-        if (i >= kBufs && !mbar_wait_soon(buf_free + buf, buf_phase ^ 1, abort_flag, p.d_status,
-                                     XAXB_DEVICE_TIMEOUT * 1000 + kSiteBlkMmaAcc))
-          break;
+      if (*abort_flag) wait_for_last_copies();
+    } else if ((warp == kPromoteWarps + 1 || warp == kPromoteWarps + 2) && lane == 0) {
+      // ------------------------------------------------------------------ MMA issuers
+      const int step = Cfg::issue_step(stages), first = warp - (kPromoteWarps + 1);
+      int stage = first, buf = first;
+      uint32_t phase = 0;
+      for (int i = first < step ? first : nkb; i < nkb; i += step) {
         if (!mbar_wait_soon(full + stage, phase, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSiteBlkMma)) break;
         tc_fence_after_sync();
         const uint64_t w_desc = umma_desc_kmajor_sw128(smem_u32(smem_w + stage * Cfg::kWeightBytes));
@@ -198,51 +219,60 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
 #pragma unroll
         for (int k = 0; k < kBKBytes / 32; ++k) umma_f8(tmem_base + buf * NT, w_desc + 2 * k, x_desc + 2 * k, kIdesc, k != 0);
         umma_commit(done + stage);
-        if (++stage == kStages) stage = 0, phase ^= 1;
-        if (++buf == kBufs) buf = 0, buf_phase ^= 1;
+        if ((stage += step) >= stages) stage -= stages, phase ^= 1;
+        if ((buf += step) >= kBufs) buf -= kBufs;
       }
     }
   } else {
-    const int quarter = warp & 3, t = threadIdx.x - 64;
-    const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16);
+    // ------------------------------------------------------------------ promotion
+    // A stage's commit barrier never completes a second time before these warps have seen the first: the block that
+    // uses the stage next waits for a buffer that they free after that (stages >= kBufs).
+    if constexpr (Cfg::kMoveRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kPromoteRegs));
+    const int quarter = warp & 3, col0 = (warp >> 2) * Cfg::kCols, t = threadIdx.x;
+    const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + col0;
     const float* b_inv = p.b_inv + (long long)tile_n * p.num_k_blocks + kb0;
-    float acc[NT];
+    float acc[Cfg::kCols];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) acc[j] = 0.0f;
-    int stage = 0, buf = 0;
+    for (int j = 0; j < Cfg::kCols; ++j) acc[j] = 0.0f;
+    int stage = 0, buf = 0, next = kBufs % stages;  // next: the stage of the block that will use this one's buffer
     uint32_t phase = 0;
     bool ok = true;
+    if (lane == 0) {  // all buffers start free
+#pragma unroll
+      for (int b = 0; b < kBufs; ++b) mbar_arrive(full + b);
+    }
+#pragma unroll 1
     for (int i = 0; i < nkb; ++i) {
       const int in_chunk = i % Cfg::kScaleBlocks;
       if (in_chunk == 0) {  // the combined multipliers of the next blocks
-        if (i > 0) promote_sync();
+        if (i > 0) promote_sync<128 * Cfg::kGroups>();
         const int n = min(Cfg::kScaleBlocks, nkb - i);
         const int m = m0 + t % NT;
         const float* a_inv = p.a_inv + (long long)m * p.num_k_blocks + kb0 + i;
 #pragma unroll 4
-        for (int b = t / NT; b < n; b += 128 / NT)
+        for (int b = t / NT; b < n; b += 128 * Cfg::kGroups / NT)
           scales[b * NT + t % NT] = m < p.M ? __ldg(a_inv + b) * __ldg(b_inv + i + b) : 0.0f;
-        promote_sync();
+        promote_sync<128 * Cfg::kGroups>();
       }
       if (!mbar_try_wait(done + stage, phase) && ok)
         ok = mbar_wait_soon(done + stage, phase, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSiteBlkPromote);
       ok = __all_sync(0xffffffffu, ok);  // (a warp that gave up still takes part in the barriers above)
       if (ok) {
         tc_fence_after_sync();
-        const float* sc = scales + in_chunk * NT;
+        const float* sc = scales + in_chunk * NT + col0;
         const uint32_t from = taddr + buf * NT;
 #pragma unroll
-        for (int c = 0; c < NT; c += Cfg::kLoad) {
+        for (int c = 0; c < Cfg::kCols; c += Cfg::kLoad) {
           uint32_t r[Cfg::kLoad];
           if constexpr (Cfg::kLoad == 32)
             tmem_ld_x32(from + c, r);
           else
             tmem_ld_x16(from + c, r);
           tmem_ld_wait();
-          if (c + Cfg::kLoad == NT) {
+          if (c + Cfg::kLoad == Cfg::kCols) {
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(buf_free + buf);
+            if (lane == 0) mbar_arrive(full + next);
           }
 #pragma unroll
           for (int j = 0; j < Cfg::kLoad; j += 4) {
@@ -252,14 +282,15 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
           }
         }
       }
-      if (++stage == kStages) stage = 0, phase ^= 1;
+      if (++stage == stages) stage = 0, phase ^= 1;
+      if (++next == stages) next = 0;
       if (++buf == kBufs) buf = 0;
     }
     // The last block's commit covers every MMA, and every MMA every copy: the ring is free.
     if (ok) {
-      float* mine = park + quarter * 32 + lane;
+      float* mine = park + col0 * Cfg::kParkFloats + quarter * 32 + lane;
 #pragma unroll
-      for (int j = 0; j < NT; ++j) mine[j * Cfg::kParkFloats] = acc[j];
+      for (int j = 0; j < Cfg::kCols; ++j) mine[j * Cfg::kParkFloats] = acc[j];
     }
     tc_fence_before_sync();
   }
@@ -269,12 +300,13 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
   else
     __syncthreads();
 
-  // This CTA adds its share of the tile's (token, 8 weight rows) items over the ranks.
-  if (!*abort_flag) {
+  // This CTA adds its share of the tile's (token, 8 weight rows) items over the ranks.  (Promoting warps only: with NT = 128
+  // the others are down to 32 registers, which only barriers can follow.)
+  if (warp < kPromoteWarps && !*abort_flag) {
     const int items = min(NT, p.M - m0) * (kBM / 8);
     const int hi = items * (rank + 1) / S;
     const uint32_t park_addr = smem_u32(park);
-    for (int it = items * rank / S + threadIdx.x; it < hi; it += kGemmThreads) {
+    for (int it = items * rank / S + threadIdx.x; it < hi; it += 32 * kPromoteWarps) {
       const int tok = it / (kBM / 8), r8 = it % (kBM / 8) * 8, n = n0 + r8;
       if (n >= p.N) continue;
       const uint32_t off = park_addr + (uint32_t)(tok * Cfg::kParkFloats + r8) * 4u;
@@ -291,7 +323,8 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
   __syncwarp();
   if (S > 1) cluster_sync_all();  // the peers have finished reading this CTA's part
   __syncthreads();
-  if (warp == 2) {
+  if (warp == kPromoteWarps + 1) {
+    if (*abort_flag) wait_for_last_copies();  // (and MMAs)
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, Cfg::kTmemCols);
   }
@@ -315,11 +348,16 @@ static int launch_decode(const Ctx* ctx, cudaStream_t stream, const GemmBlocksPa
   CUtensorMap tw, tx;
   if (int rc = make_tmap_2d(ctx, &tw, p.b, 1, (uint64_t)p.K, (uint64_t)p.N, (uint64_t)p.ldb, kBKBytes, kBM)) return rc;
   if (int rc = make_tmap_2d(ctx, &tx, p.a, 1, (uint64_t)p.K, (uint64_t)p.M, (uint64_t)p.lda, kBKBytes, NT)) return rc;
-  if (int rc = ensure_dynamic_smem<gemm_blocks_decode_kernel<NT>>(ctx, Cfg::kSmemBytes, "gemm_blocks_decode_kernel")) return rc;
+  if (int rc = ensure_dynamic_smem<gemm_blocks_decode_kernel<NT>>(ctx, Cfg::smem_bytes(Cfg::stages_for(1)),
+                                                                  "gemm_blocks_decode_kernel"))
+    return rc;
   const int tiles_n = (p.N + kBM - 1) / kBM, tiles_m = (p.M + NT - 1) / NT;
   const int S = pick_split(tiles_n * tiles_m, p.num_k_blocks, ctx->num_sms);
+  const long long ctas = (long long)tiles_n * tiles_m * S;
+  const int per_sm = (int)min((long long)Cfg::kCtasPerSm, (ctas + ctx->num_sms - 1) / ctx->num_sms);
+  const int stages = Cfg::stages_for(per_sm);
   cudaError_t e = launch_kernel(gemm_blocks_decode_kernel<NT>, dim3((unsigned)(tiles_n * S), (unsigned)tiles_m),
-                                dim3(kGemmThreads), Cfg::kSmemBytes, stream, (unsigned)S, tw, tx, p, S);
+                                dim3(Cfg::kThreads), Cfg::smem_bytes(stages), stream, (unsigned)S, tw, tx, p, S, stages);
   if (e != cudaSuccess) {
     set_last_error("gemm_blocks_decode_kernel launch: %s", cudaGetErrorString(e));
     return XAXB_LAUNCH_FAILED;
@@ -347,6 +385,7 @@ constexpr int kPairLaunchRegs = 168, kPairPromoteRegs = 192, kPairIssueRegs = 12
 static_assert(2 * kPairPromoteRegs + kPairIssueRegs <= 3 * kPairLaunchRegs, "register split");
 constexpr int kPairTile = 256;
 constexpr int kPairStages = 5;
+static_assert(kPairStages >= 2 + 2, "two issuing threads on a ring of odd length: see BlocksDecodeCfg::issue_step");
 constexpr int kPairOperandBytes = kBM * kBKBytes;          // per CTA, operand and stage
 constexpr int kPairStageBytes = 2 * kPairOperandBytes;
 constexpr int kPairOutBytes = kBM * 128;                   // 128 rows of 64 bf16: one TMA store
@@ -441,11 +480,7 @@ gemm_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
             if (++stage == kPairStages) stage = 0, phase ^= 1;
           }
         }
-        if (!ok) {  // given up: nothing has moved for the wait limit; a millisecond more for the copies asked for last
-          const unsigned long long t0 = globaltimer_ns();
-          while (globaltimer_ns() - t0 < 1000000ull) {
-          }
-        }
+        if (!ok) wait_for_last_copies();
       }
     } else if (warp <= 10 && rank == 0) {
       // ---------------------------------------------------------------- MMA issuers (leader only)
