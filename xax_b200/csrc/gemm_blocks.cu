@@ -50,14 +50,9 @@ __device__ __forceinline__ void wait_for_last_copies() {
   }
 }
 
-// Distributed-shared-memory load that stays behind the barrier in front of it.
-__device__ __forceinline__ float4 ld_dsmem_f4_ordered(uint32_t cluster_addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(cluster_addr)
-               : "memory");
-  return v;
+// A store into the shared memory of a CTA of the cluster.
+__device__ __forceinline__ void st_dsmem_f4(uint32_t cluster_addr, float a, float b, float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
 
 // Barrier over one warpgroup of the pair kernel (two of them promote).
@@ -97,12 +92,14 @@ __device__ __forceinline__ void fma2(float& a, float& b, uint32_t x, uint32_t y,
 }
 
 // ---------------------------------------------------------------------------------------
-// Few rows: weight streaming.  The weights are the MMA's 128-row operand and NT rows of activations its columns, so a
-// decode step moves 16 KB of weights and only NT * 128 bytes of activations per K block.  A cluster of S CTAs shares
-// the K blocks of one tile; each CTA leaves its part of the result in shared memory and the cluster adds the parts
-// over distributed shared memory in rank order (no atomics: the same bits every time).
-//   promoting warps  thread = weight row; acc[t] += partial[t] * (a_inv[t, kb] * b_inv[kb]) in float32 registers, up to
-//                    64 tokens a thread (two warpgroups for NT = 128)
+// Few rows: weight streaming.  For up to 64 tokens the weights are the MMA's 128-row operand and NT rows of activations its
+// columns, so a decode step moves 16 KB of weights and only NT * 128 bytes of activations per K block.  A cluster of S
+// CTAs shares the K blocks of one tile; each CTA pushes its part of the result into the shared memory of the CTA that
+// owns the token, which adds the parts in rank order (no atomics: the same bits every time).  (Pulling the parts took
+// S remote round trips per item: 7000 of 38000 cycles for 128 x 4096 x 14336, S = 4.)
+//   promoting warps  thread = weight row; acc[t] += partial[t] * (a_inv[t, kb] * b_inv[kb]) in float32 registers.  With
+//                    NT = 128 the operands change places: thread = token, two warpgroups of 64 weight rows each, and the
+//                    combined multiplier is one value a thread instead of one a column.
 //   next warp        TMA producer (weight and activation tiles into a ring)
 //   next two warps   one thread each issues the four MMAs of every other K block into the next tensor-memory buffer (one
 //                    thread those of all blocks where the ring is too short for two, see issue_step)
@@ -114,15 +111,16 @@ __device__ __forceinline__ void fma2(float& a, float& b, uint32_t x, uint32_t y,
 // which will be resident together leave (`stages`, from the launcher).
 template <int NT>
 struct BlocksDecodeCfg {
+  static constexpr bool kTokenRows = NT == 128;            // the token is the accumulator's row, else the weight row is
   static constexpr int kGroups = NT == 128 ? 2 : 1;        // promoting warpgroups
-  static constexpr int kCols = NT / kGroups;               // tokens per promoting thread
+  static constexpr int kCols = NT / kGroups;               // accumulator columns per promoting thread
   static constexpr int kThreads = NT == 128 ? 384 : 224;
   // Registers of NT = 128: two CTAs of 384 threads start with 80 a thread; the warpgroup of the producer and the
   // issuer gives up what the promoting ones need.
   static constexpr bool kMoveRegs = NT == 128;
   static constexpr int kPromoteRegs = 104, kIssueRegs = 32;
   static_assert(kGroups * kPromoteRegs + kIssueRegs <= 3 * 80, "register split");
-  static constexpr int kCtasPerSm = NT <= 32 ? 3 : 2;      // at most: registers, tensor memory
+  static constexpr int kCtasPerSm = NT == 16 ? 3 : 2;      // at most: registers, tensor memory
   static constexpr int kWeightBytes = kBM * kBKBytes;
   static constexpr int kStageBytes = kWeightBytes + NT * kBKBytes;
   static constexpr int kMaxStages = 12;
@@ -130,7 +128,7 @@ struct BlocksDecodeCfg {
   static constexpr int kTmemCols = NT == 32 ? 128 : kBufs * NT;
   static constexpr int kScaleBlocks = 16;                  // K blocks whose multipliers are staged at a time
   static constexpr int kLoad = NT == 16 || NT == 128 ? 16 : 32;  // columns per readout (what the registers allow)
-  static constexpr int kParkFloats = kBM + 4;              // floats per token of the parked result
+  static constexpr int kPartFloats = kBM + 4;              // floats per token of a CTA's part of the result
   static constexpr int kExtraBytes = kScaleBlocks * NT * 4 + (2 * kMaxStages + 1) * 8;
   static constexpr int kSmemPerSm = 228 * 1024, kSmemReserved = 1024;
   // The ring that leaves room for `ctas` CTAs on an SM, and for no more of them than tensor memory serves.
@@ -143,7 +141,7 @@ struct BlocksDecodeCfg {
   // is the same thread's (stages even).
   static constexpr int issue_step(int stages) { return stages % 2 == 0 || stages >= kBufs + 2 ? 2 : 1; }
   static constexpr int smem_bytes(int stages) { return stages * kStageBytes + kExtraBytes; }
-  static_assert(NT * kParkFloats * 4 <= 3 * kStageBytes, "the parked result overlays the ring");
+  static_assert((kTokenRows ? 1 : 2) * NT * kPartFloats * 4 <= 3 * kStageBytes, "the parts overlay the ring");
   static_assert(stages_for(kCtasPerSm) >= kBufs && stages_for(kCtasPerSm) >= 3, "a stage comes round no sooner than a buffer");
   static_assert(kCtasPerSm * kTmemCols <= 512, "tensor memory");
 };
@@ -159,7 +157,7 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
   uint8_t* smem_w = smem;
   uint8_t* smem_x = smem + stages * Cfg::kWeightBytes;
   float* scales = reinterpret_cast<float*>(smem + stages * Cfg::kStageBytes);  // [kScaleBlocks][NT]
-  float* park = reinterpret_cast<float*>(smem);                                // [NT][kParkFloats], after the main loop
+  float* parts = reinterpret_cast<float*>(smem);  // after the main loop: [S][NT / S][kPartFloats], this CTA's tokens
   uint64_t* full = reinterpret_cast<uint64_t*>(scales + Cfg::kScaleBlocks * NT);  // [stages]
   uint64_t* done = full + Cfg::kMaxStages;                                     // [stages]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + Cfg::kMaxStages);
@@ -217,7 +215,9 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
         const uint64_t w_desc = umma_desc_kmajor_sw128(smem_u32(smem_w + stage * Cfg::kWeightBytes));
         const uint64_t x_desc = umma_desc_kmajor_sw128(smem_u32(smem_x + stage * NT * kBKBytes));
 #pragma unroll
-        for (int k = 0; k < kBKBytes / 32; ++k) umma_f8(tmem_base + buf * NT, w_desc + 2 * k, x_desc + 2 * k, kIdesc, k != 0);
+        for (int k = 0; k < kBKBytes / 32; ++k)
+          umma_f8(tmem_base + buf * NT, (Cfg::kTokenRows ? x_desc : w_desc) + 2 * k, (Cfg::kTokenRows ? w_desc : x_desc) + 2 * k,
+                  kIdesc, k != 0);
         umma_commit(done + stage);
         if ((stage += step) >= stages) stage -= stages, phase ^= 1;
         if ((buf += step) >= kBufs) buf -= kBufs;
@@ -230,7 +230,6 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
     if constexpr (Cfg::kMoveRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kPromoteRegs));
     const int quarter = warp & 3, col0 = (warp >> 2) * Cfg::kCols, t = threadIdx.x;
     const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + col0;
-    const float* b_inv = p.b_inv + (long long)tile_n * p.num_k_blocks + kb0;
     float acc[Cfg::kCols];
 #pragma unroll
     for (int j = 0; j < Cfg::kCols; ++j) acc[j] = 0.0f;
@@ -246,12 +245,17 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
       const int in_chunk = i % Cfg::kScaleBlocks;
       if (in_chunk == 0) {  // the combined multipliers of the next blocks
         if (i > 0) promote_sync<128 * Cfg::kGroups>();
-        const int n = min(Cfg::kScaleBlocks, nkb - i);
-        const int m = m0 + t % NT;
-        const float* a_inv = p.a_inv + (long long)m * p.num_k_blocks + kb0 + i;
-#pragma unroll 4
-        for (int b = t / NT; b < n; b += 128 * Cfg::kGroups / NT)
-          scales[b * NT + t % NT] = m < p.M ? __ldg(a_inv + b) * __ldg(b_inv + i + b) : 0.0f;
+        constexpr int kEach = Cfg::kScaleBlocks * NT / (128 * Cfg::kGroups);  // a thread's, all asked for at once
+        const int m = min(m0 + t % NT, p.M - 1), b0 = t / NT * kEach;         // (rows past M are never stored)
+        const float *a_inv = p.a_inv + (long long)m * p.num_k_blocks + kb0, *b_inv = p.b_inv + (long long)tile_n * p.num_k_blocks + kb0;
+        float v[kEach], w[kEach];
+#pragma unroll
+        for (int b = 0; b < kEach; ++b) {
+          const int at = min(i + b0 + b, nkb - 1);
+          v[b] = __ldg(a_inv + at), w[b] = __ldg(b_inv + at);
+        }
+#pragma unroll
+        for (int b = 0; b < kEach; ++b) scales[(b0 + b) * NT + t % NT] = v[b] * w[b];
         promote_sync<128 * Cfg::kGroups>();
       }
       if (!mbar_try_wait(done + stage, phase) && ok)
@@ -259,7 +263,8 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
       ok = __all_sync(0xffffffffu, ok);  // (a warp that gave up still takes part in the barriers above)
       if (ok) {
         tc_fence_after_sync();
-        const float* sc = scales + in_chunk * NT + col0;
+        const float* sc = scales + in_chunk * NT + (Cfg::kTokenRows ? quarter * 32 + lane : 0);
+        const float row_scale = Cfg::kTokenRows ? *sc : 0.0f;
         const uint32_t from = taddr + buf * NT;
 #pragma unroll
         for (int c = 0; c < Cfg::kCols; c += Cfg::kLoad) {
@@ -276,7 +281,8 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
           }
 #pragma unroll
           for (int j = 0; j < Cfg::kLoad; j += 4) {
-            const float4 s4 = *reinterpret_cast<const float4*>(sc + c + j);
+            const float4 s4 = Cfg::kTokenRows ? make_float4(row_scale, row_scale, row_scale, row_scale)
+                                              : *reinterpret_cast<const float4*>(sc + c + j);
             fma2(acc[c + j], acc[c + j + 1], r[j], r[j + 1], s4.x, s4.y);
             fma2(acc[c + j + 2], acc[c + j + 3], r[j + 2], r[j + 3], s4.z, s4.w);
           }
@@ -286,42 +292,65 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
       if (++next == stages) next = 0;
       if (++buf == kBufs) buf = 0;
     }
-    // The last block's commit covers every MMA, and every MMA every copy: the ring is free.
-    if (ok) {
-      float* mine = park + col0 * Cfg::kParkFloats + quarter * 32 + lane;
+    // Every block is done, and with it every copy: this CTA's ring is free.  Threads whose row is a token hold neighbouring
+    // columns and can push 16 bytes at a time; the others first turn their part round in shared memory (scalar pushes
+    // were slower than all of it: 20 us against 9 for 64 x 2048 x 5632).
+    const int per = NT / S, tokens = min(NT, p.M - m0);  // tokens per owner (a power of two); those that exist
+    const int row = quarter * 32 + lane;
+    float* turned = Cfg::kTokenRows || S == 1 ? parts : parts + NT * Cfg::kPartFloats;
+    if (!Cfg::kTokenRows && ok) {
 #pragma unroll
-      for (int j = 0; j < Cfg::kCols; ++j) mine[j * Cfg::kParkFloats] = acc[j];
+      for (int j = 0; j < Cfg::kCols; ++j)
+        if (j < tokens) turned[j * Cfg::kPartFloats + row] = acc[j];
     }
     tc_fence_before_sync();
-  }
-  __syncwarp();
-  if (S > 1)
-    cluster_sync_all();  // every CTA's part is visible to the cluster
-  else
-    __syncthreads();
-
-  // This CTA adds its share of the tile's (token, 8 weight rows) items over the ranks.  (Promoting warps only: with NT = 128
-  // the others are down to 32 registers, which only barriers can follow.)
-  if (warp < kPromoteWarps && !*abort_flag) {
-    const int items = min(NT, p.M - m0) * (kBM / 8);
-    const int hi = items * (rank + 1) / S;
-    const uint32_t park_addr = smem_u32(park);
-    for (int it = items * rank / S + threadIdx.x; it < hi; it += 32 * kPromoteWarps) {
-      const int tok = it / (kBM / 8), r8 = it % (kBM / 8) * 8, n = n0 + r8;
-      if (n >= p.N) continue;
-      const uint32_t off = park_addr + (uint32_t)(tok * Cfg::kParkFloats + r8) * 4u;
-      float f[8] = {};
-      for (int src = 0; src < S; ++src) {
-        const uint32_t at = S > 1 ? dsmem_addr(off, (uint32_t)src) : off;
-        const float4 lo = ld_dsmem_f4_ordered(at), hi4 = ld_dsmem_f4_ordered(at + 16);
-        f[0] += lo.x, f[1] += lo.y, f[2] += lo.z, f[3] += lo.w;
-        f[4] += hi4.x, f[5] += hi4.y, f[6] += hi4.z, f[7] += hi4.w;
+    __syncwarp();
+    if (S > 1)
+      cluster_sync_all();  // the rings of the whole cluster are free
+    else
+      promote_sync<128 * Cfg::kGroups>();
+    if (ok && Cfg::kTokenRows && row < tokens) {
+      const uint32_t mine = smem_u32(parts) + (uint32_t)((rank * per + row % per) * Cfg::kPartFloats + col0) * 4u;
+      const uint32_t at = S > 1 ? dsmem_addr(mine, (uint32_t)(row / per)) : mine;
+#pragma unroll
+      for (int j = 0; j < Cfg::kCols; j += 4) st_dsmem_f4(at + j * 4, acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+    } else if (ok && !Cfg::kTokenRows && S > 1) {
+      for (int it = t; it < tokens * (kBM / 4); it += 128 * Cfg::kGroups) {
+        const int tok = it / (kBM / 4), r4 = it % (kBM / 4) * 4;
+        const float4 v = *reinterpret_cast<const float4*>(turned + tok * Cfg::kPartFloats + r4);
+        const uint32_t mine = smem_u32(parts) + (uint32_t)((rank * per + tok % per) * Cfg::kPartFloats + r4) * 4u;
+        st_dsmem_f4(dsmem_addr(mine, (uint32_t)(tok / per)), v.x, v.y, v.z, v.w);
       }
-      finish8(p, f, m0 + tok, n);
+    }
+    if (S > 1)
+      cluster_sync_all();  // every part has arrived
+    else
+      promote_sync<128 * Cfg::kGroups>();
+    if (!*abort_flag) {
+      const int items = min(per, tokens - rank * per) * (kBM / 8);
+      for (int it = t; it < items; it += 128 * Cfg::kGroups) {
+        const int tok = it / (kBM / 8), r8 = it % (kBM / 8) * 8, n = n0 + r8;
+        if (n >= p.N) continue;
+        const float* from = parts + tok * Cfg::kPartFloats + r8;
+        float f[8] = {};
+#pragma unroll
+        for (int src = 0; src < 8; ++src) {
+          if (src < S) {
+            const float4 lo = *reinterpret_cast<const float4*>(from + src * per * Cfg::kPartFloats);
+            const float4 hi = *reinterpret_cast<const float4*>(from + src * per * Cfg::kPartFloats + 4);
+            f[0] += lo.x, f[1] += lo.y, f[2] += lo.z, f[3] += lo.w;
+            f[4] += hi.x, f[5] += hi.y, f[6] += hi.z, f[7] += hi.w;
+          }
+        }
+        finish8(p, f, m0 + rank * per + tok, n);
+      }
     }
   }
-  __syncwarp();
-  if (S > 1) cluster_sync_all();  // the peers have finished reading this CTA's part
+  if (warp >= kPromoteWarps && S > 1) {  // the two barriers of the cluster above (barriers are all that may follow here:
+    __syncwarp();                        // with NT = 128 these warps are down to 32 registers)
+    cluster_sync_all();
+    cluster_sync_all();
+  }
   __syncthreads();
   if (warp == kPromoteWarps + 1) {
     if (*abort_flag) wait_for_last_copies();  // (and MMAs)
@@ -330,16 +359,14 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
   }
 }
 
-// How many CTAs share a tile's K blocks.
-static int pick_split(int tiles, int num_k_blocks, int num_sms) {
-  int best = 1;
-  double best_t = 1e30;
-  for (int s = 1; s <= 8 && s <= num_k_blocks; ++s) {
-    const double per_sm = (tiles * s + num_sms - 1) / num_sms;
-    const double t = per_sm * ((num_k_blocks + s - 1) / s) * 0.37 + (s > 1 ? 1.5 + 0.1 * s : 0.0);
-    if (t < best_t) best_t = t, best = s;
-  }
-  return best;
+// How many CTAs share a tile's K blocks: as many as keep one CTA on an SM, since what a second one brings is less than the
+// cluster's two barriers and pushes cost (64 x 28672 x 4096, 224 tiles: 24.9 us undivided, 33.0 with two; 16 x 6144 x 4096,
+// 48 tiles: 11.1, 8.0 and 7.9 us with 1, 2 and 4).  Clusters of eight find room for their CTAs on one SM each in few places
+// (64 x 2048 x 5632, 16 tiles: 8.6 us with 4, 13.3 with 8), so they are for few tiles; a CTA keeps four blocks at least.
+static int pick_split(long long tiles, int num_k_blocks, int num_sms) {
+  int s = 1;
+  while (s < 8 && tiles * s * 2 <= (s == 4 ? 64 : num_sms) && num_k_blocks >= 8 * s) s *= 2;
+  return s;
 }
 
 template <int NT>
@@ -352,7 +379,7 @@ static int launch_decode(const Ctx* ctx, cudaStream_t stream, const GemmBlocksPa
                                                                   "gemm_blocks_decode_kernel"))
     return rc;
   const int tiles_n = (p.N + kBM - 1) / kBM, tiles_m = (p.M + NT - 1) / NT;
-  const int S = pick_split(tiles_n * tiles_m, p.num_k_blocks, ctx->num_sms);
+  const int S = pick_split((long long)tiles_n * tiles_m, p.num_k_blocks, ctx->num_sms);
   const long long ctas = (long long)tiles_n * tiles_m * S;
   const int per_sm = (int)min((long long)Cfg::kCtasPerSm, (ctas + ctx->num_sms - 1) / ctx->num_sms);
   const int stages = Cfg::stages_for(per_sm);
@@ -758,7 +785,9 @@ extern "C" int xaxb_gemm_fp8_blocks(xaxb_ctx* ctx_, void* stream, const void* a_
     set_last_error("gemm_fp8_blocks: [%lld, %lld] has too many tiles", (long long)M, (long long)N);
     return XAXB_BAD_ARGUMENT;
   }
-  if (M > 128 && 2 * pair_tiles >= ctx->num_sms) return launch_pair(ctx, s, p);
+  // The pair kernel from where 128 x 128 tiles no longer fit one on an SM: 512 x 4096 x 4096 (128 tiles) 17.9 us on them and
+  // 19.1 on pairs, 768 x 4096 x 4096 (192 tiles) 26.9 and 20.2, 256 x 28672 x 4096 52.4 and 35.9.
+  if (M > 128 && ((M + kBM - 1) / kBM) * ((N + kBM - 1) / kBM) > ctx->num_sms) return launch_pair(ctx, s, p);
   if (M <= 16) return launch_decode<16>(ctx, s, p);
   if (M <= 32) return launch_decode<32>(ctx, s, p);
   if (M <= 64) return launch_decode<64>(ctx, s, p);
