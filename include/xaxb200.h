@@ -170,8 +170,8 @@ int xaxb_gemm_fp8_formats(xaxb_ctx* ctx, void* stream, const void* a_fp8, int64_
  *   a[m, k] * b[n, k]) + bias[n] + residual[m, n] ), sums in float32; a_inv, b_inv contiguous; bias bf16 [N] or NULL,
  *   residual bf16 [M, ldr] or NULL.
  *
- * Tensors are contiguous unless a stride is given and 16-byte aligned; cols, dim, K, lda and ldb are multiples of 16,
- * N, ld, ldr and ldo of 8.
+ * Tensors are contiguous unless a stride is given and 16-byte aligned, the bf16 tensors of the three casts 32-byte
+ * aligned; cols, dim, ld, K, lda and ldb are multiples of 16, N, ldr and ldo of 8.
  */
 int xaxb_quantize_blocks(xaxb_ctx* ctx, void* stream, const void* x_bf16, int64_t rows, int64_t cols, int block_rows,
                          void* q_e4m3, float* inv_scale);

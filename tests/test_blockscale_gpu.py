@@ -392,10 +392,17 @@ def test_empty_and_copied_inputs():
     assert ops.gemm_fp8_blocks(q, b_q, inv, b_inv).shape == (0, 264)
     # a transposed or sliced input is copied, like the other operators do it
     y = activations(256, 64, 3)
-    for view in (y.t(), y[:, 16:48], activations(8, 512, 4)[:, ::2]):
+    odd = y.reshape(-1)[4:4 + 512].reshape(2, 256)  # contiguous, 8 bytes off the boundary that the kernels load at
+    for view in (y.t(), y[:, 16:48], activations(8, 512, 4)[:, ::2], odd):
         got, want = ops.quantize_blocks(view), ops.quantize_blocks(view.contiguous())
         same_bytes(got[0], want[0])
         assert torch.equal(got[1], want[1])
+    w = torch.ones((257,), dtype=BF16, device="cuda")
+    for got, want in zip(ops.rmsnorm_blocks(odd, w[1:], 1e-6, residual=odd),
+                         ops.rmsnorm_blocks(odd.clone(), w[:256], 1e-6, residual=odd.clone())):
+        assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
+    for got, want in zip(ops.silu_mul_blocks(odd, 128), ops.silu_mul_blocks(odd.clone(), 128)):
+        assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
 
 
 def test_arguments_are_checked():
@@ -408,7 +415,6 @@ def test_arguments_are_checked():
     bad = [
         lambda: ops.quantize_blocks(x.float()), lambda: ops.quantize_blocks(x[0]), lambda: ops.quantize_blocks(x, 64),
         lambda: ops.quantize_blocks(x[:, :24].contiguous()), lambda: ops.quantize_blocks(x[:, :0]),
-        lambda: ops.quantize_blocks(x.reshape(-1)[4:4 + 256].reshape(1, 256)),  # 8 bytes off the 16-byte boundary
         lambda: ops.rmsnorm_blocks(x, w[:128], 1e-6), lambda: ops.rmsnorm_blocks(x, w.float(), 1e-6),
         lambda: ops.rmsnorm_blocks(x, w, 1e-6, residual=x[:2]),
         lambda: ops.silu_mul_blocks(x, 256), lambda: ops.silu_mul_blocks(x, 0), lambda: ops.silu_mul_blocks(x, 100),

@@ -164,6 +164,14 @@ def stream_ptr() -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
+def call_state(device: int):
+    """(context, stream handle, library) for a call on ``device``, the current one: ctx, stream_ptr and load in one."""
+    import torch
+
+    h = _ctxs.get(device)
+    return ctx(device) if h is None else h, torch._C._cuda_getCurrentRawStream(device), _lib if _lib is not None else load()
+
+
 def check(rc: int, what: str) -> None:
     """Map a status code to the exception the reference would raise for the same condition."""
     if rc == OK:

@@ -8,8 +8,9 @@
 // so the block stands for q * inv.  Everything between the bf16 inputs and q is float32: one rounding to 8 bits at
 // the end (the floor of 2^-126 keeps 1/inv finite; with it the largest value of a normal block lands on 448).
 //
-// All are bandwidth kernels.  A thread owns 16 consecutive values (two 16-byte loads, one 16-byte store), so the
-// eight threads of a block of 128 are eight neighbouring lanes and its maximum takes three shuffles.
+// All are bandwidth kernels.  A thread owns 16 consecutive values: one 32-byte load (half the load instructions of two
+// 16-byte ones, and whole sectors), one 16-byte store; the eight threads of a block of 128 are eight neighbouring lanes
+// and its maximum takes three shuffles.
 #include "common.cuh"
 #include "quant_device.cuh"
 
@@ -18,14 +19,39 @@ namespace xaxb {
 constexpr int kPiece = 16;               // values per thread and piece
 constexpr int kBlockPieces = 128 / kPiece;
 
-// Magnitudes compare as unsigned bit patterns, which puts NaN above infinity: a NaN in a block reaches its amax.
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+struct Packed16 {  // 16 bf16
+  uint32_t w[8];
+};
 
+__device__ __forceinline__ Packed16 load16(const __nv_bfloat16* p) {
+  Packed16 r;
+  asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7])
+               : "l"(p));
+  return r;
+}
+
+__device__ __forceinline__ void store16(__nv_bfloat16* p, const Packed16& r) {
+  asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
+               ::"r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]), "r"(r.w[3]), "r"(r.w[4]), "r"(r.w[5]), "r"(r.w[6]), "r"(r.w[7]), "l"(p)
+               : "memory");
+}
+
+__device__ __forceinline__ float low(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+// Magnitudes compare as unsigned bit patterns, which puts NaN above infinity: a NaN in a block reaches its amax.
 __device__ __forceinline__ uint32_t magnitude16(const float (&v)[kPiece]) {
   uint32_t m = 0;
 #pragma unroll
-  for (int j = 0; j < kPiece; ++j) m = max(m, magnitude(v[j]));
+  for (int j = 0; j < kPiece; ++j) m = max(m, __float_as_uint(v[j]) & 0x7FFFFFFFu);
   return m;
+}
+__device__ __forceinline__ uint32_t magnitude16(const Packed16& p) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = __vmaxu2(m, p.w[j] & 0x7FFF7FFFu);
+  return max(m << 16, m & 0xFFFF0000u);
 }
 
 __device__ __forceinline__ uint32_t lanes8_max(uint32_t m) {
@@ -46,19 +72,11 @@ __device__ __forceinline__ uint4 cast16(const float (&v)[kPiece], float scale) {
     w[j] = e4m3x2(v[4 * j] * scale, v[4 * j + 1] * scale) | (e4m3x2(v[4 * j + 2] * scale, v[4 * j + 3] * scale) << 16);
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-
-__device__ __forceinline__ void load16(const __nv_bfloat16* p, float (&v)[kPiece]) {
-  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
-  float lo[8], hi[8];
-  unpack8(a, lo);
-  unpack8(b, hi);
+__device__ __forceinline__ uint4 cast16(const Packed16& p, float scale) {
+  float v[kPiece];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = lo[j], v[8 + j] = hi[j];
-}
-
-__device__ __forceinline__ void zero16(float (&v)[kPiece]) {
-#pragma unroll
-  for (int j = 0; j < kPiece; ++j) v[j] = 0.0f;
+  for (int j = 0; j < 8; ++j) v[2 * j] = low(p.w[j]), v[2 * j + 1] = high(p.w[j]);
+  return cast16(v, scale);
 }
 
 // n / d for n < 2^31 by a multiplication with a precomputed reciprocal: with l = ceil(log2 d) and
@@ -79,14 +97,13 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const __nv_bfloat1
                                                               FastDiv per_row, int cols, uint8_t* __restrict__ q,
                                                               float* __restrict__ inv) {
   pdl_trigger();
-  pdl_wait();
   const uint32_t p = blockIdx.x * 256u + threadIdx.x;
   const uint32_t row = div_by(p, per_row), col = (p - row * per_row.d) * kPiece;
   const bool here = p < pieces && col < (uint32_t)cols;
   const int64_t at = (int64_t)row * cols + col;
-  float v[kPiece];
-  zero16(v);
-  if (here) load16(x + at, v);
+  pdl_wait();
+  Packed16 v = {};
+  if (here) v = load16(x + at);
   const float s = block_inv_scale(lanes8_max(magnitude16(v)));
   if (here) {
     *reinterpret_cast<uint4*>(q + at) = cast16(v, 1.0f / s);
@@ -94,73 +111,92 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const __nv_bfloat1
   }
 }
 
-// ---- 128 x 128 squares: one CTA each, four pieces per thread kept in registers across the maximum.
+// ---- 128 x 128 squares: one CTA each, four pieces per thread kept (packed) in registers across the maximum.
 __global__ void __launch_bounds__(256) quantize_squares_kernel(const __nv_bfloat16* __restrict__ x, int64_t rows, int cols,
                                                                uint8_t* __restrict__ q, float* __restrict__ inv) {
   pdl_trigger();
-  pdl_wait();
+  __shared__ uint32_t warp_max[8];
   const int64_t row0 = (int64_t)blockIdx.x * 128 + threadIdx.x / kBlockPieces;
   const int col = blockIdx.y * 128 + (threadIdx.x % kBlockPieces) * kPiece;
-  float v[4][kPiece];
-  uint32_t m = 0;
+  pdl_wait();
+  Packed16 v[4];
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
-    zero16(v[u]);
-    if (row0 + u * 32 < rows && col < cols) load16(x + (row0 + u * 32) * cols + col, v[u]);
-    m = max(m, magnitude16(v[u]));
+    v[u] = {};
+    if (row0 + u * 32 < rows && col < cols) v[u] = load16(x + (row0 + u * 32) * cols + col);
   }
-  const float s = block_inv_scale(block_max_u32(m));
-  const float r = 1.0f / s;
+  uint32_t m = 0;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) m = max(m, magnitude16(v[u]));
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (threadIdx.x % 32 == 0) warp_max[threadIdx.x / 32] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, warp_max[i]);
+  const float s = block_inv_scale(m), r = 1.0f / s;
 #pragma unroll
   for (int u = 0; u < 4; ++u)
     if (row0 + u * 32 < rows && col < cols) *reinterpret_cast<uint4*>(q + (row0 + u * 32) * cols + col) = cast16(v[u], r);
   if (threadIdx.x == 0) inv[(int64_t)blockIdx.x * gridDim.y + blockIdx.y] = s;
 }
 
-// ---- RMSNorm of x (+ residual): t = x + residual and the norm in float32, one CTA per row, the row in registers.
+// ---- RMSNorm of x (+ residual): t = x + residual and the norm in float32, one CTA per row, the row in registers.  A row
+// is one dependent chain (load, sum over the CTA, normalise, maximum, store), so an SM overlaps as many as it has CTAs:
+// many rows run narrow CTAs with more pieces per thread, few rows spread over more threads.
 template <int NP, int NT>
 __global__ void __launch_bounds__(NT) rmsnorm_blocks_kernel(const __nv_bfloat16* __restrict__ x,
                                                             const __nv_bfloat16* __restrict__ residual,
                                                             const __nv_bfloat16* __restrict__ weight, float eps, int cols,
-                                                            int blocks, uint4* __restrict__ sum, uint8_t* __restrict__ q,
-                                                            float* __restrict__ inv) {
+                                                            int blocks, __nv_bfloat16* __restrict__ sum,
+                                                            uint8_t* __restrict__ q, float* __restrict__ inv) {
   pdl_trigger();
-  pdl_wait();
+  __shared__ float warp_sum[NT / 32];
   const int64_t row = blockIdx.x;
+  pdl_wait();
+  constexpr bool kWeightEarly = NP <= 2;  // off the chain behind the sum, where registers allow
+  Packed16 px[NP], pr[NP], pw[NP];
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    const int col = (threadIdx.x + k * NT) * kPiece;
+    px[k] = {}, pr[k] = {};
+    if (col < cols) px[k] = load16(x + row * cols + col);
+    if (col < cols && residual) pr[k] = load16(residual + row * cols + col);
+    if (col < cols && kWeightEarly) pw[k] = load16(weight + col);
+  }
   float v[NP][kPiece];
   float ss = 0.0f;
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
     const int col = (threadIdx.x + k * NT) * kPiece;
-    zero16(v[k]);
-    if (col < cols) {
-      const int64_t at = row * cols + col;
-      load16(x + at, v[k]);
-      if (residual) {
-        float r[kPiece];
-        load16(residual + at, r);
-        float lo[8], hi[8];
+    Packed16 total;
 #pragma unroll
-        for (int j = 0; j < kPiece; ++j) {
-          v[k][j] += r[j];
-          (j < 8 ? lo[j & 7] : hi[j & 7]) = v[k][j];
-        }
-        sum[at / 8] = pack8(lo);
-        sum[at / 8 + 1] = pack8(hi);
-      }
-#pragma unroll
-      for (int j = 0; j < kPiece; ++j) ss = fmaf(v[k][j], v[k][j], ss);
+    for (int j = 0; j < 8; ++j) {
+      v[k][2 * j] = low(px[k].w[j]) + low(pr[k].w[j]);
+      v[k][2 * j + 1] = high(px[k].w[j]) + high(pr[k].w[j]);
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(total.w[j]) : "f"(v[k][2 * j + 1]), "f"(v[k][2 * j]));
     }
+    if (col < cols && residual) store16(sum + row * cols + col, total);
+#pragma unroll
+    for (int j = 0; j < kPiece; ++j) ss = fmaf(v[k][j], v[k][j], ss);
   }
-  const float n = rsqrtf(block_sum_f32(ss) / (float)cols + eps);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (threadIdx.x % 32 == 0) warp_sum[threadIdx.x / 32] = ss;
+  __syncthreads();
+  ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NT / 32; ++i) ss += warp_sum[i];
+  const float n = rsqrtf(ss / (float)cols + eps);
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
     const int piece = threadIdx.x + k * NT, col = piece * kPiece;
     if (col < cols) {
-      float w[kPiece];
-      load16(weight + col, w);
+      const Packed16 w = kWeightEarly ? pw[k] : load16(weight + col);
 #pragma unroll
-      for (int j = 0; j < kPiece; ++j) v[k][j] = v[k][j] * n * w[j];
+      for (int j = 0; j < 8; ++j) {
+        v[k][2 * j] *= n * low(w.w[j]);
+        v[k][2 * j + 1] *= n * high(w.w[j]);
+      }
     }
     const float s = block_inv_scale(lanes8_max(magnitude16(v[k])));
     if (col < cols) {
@@ -171,22 +207,38 @@ __global__ void __launch_bounds__(NT) rmsnorm_blocks_kernel(const __nv_bfloat16*
 }
 
 // ---- silu(gate) * up, gate and up the two halves of a row of the fused gate | up product.
+
+// 1 / (1 + e^-g) to a few units: e^-g = 2^h (1 + l ln 2) with h + l = -g log2 e to twice the precision, from the
+// approximate exponential and reciprocal (2^-22 each).  Below -87 the exponential nears the end of its range and the
+// result is 0 in float32 to every purpose; NaN passes through the product with g.
+__device__ __forceinline__ float sigmoid(float g) {
+  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+  const float x = -fmaxf(g, -87.0f), h = x * kLog2e, l = fmaf(x, kLog2e, -h);
+  float e, r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(h));
+  e = fmaf(e, l * kLn2, e);
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return g < -87.0f ? 0.0f : r;
+}
+
 __global__ void __launch_bounds__(256) silu_mul_blocks_kernel(const __nv_bfloat16* __restrict__ gate_up, int64_t ld,
                                                               uint32_t pieces, FastDiv per_row, int dim,
                                                               uint8_t* __restrict__ q, float* __restrict__ inv) {
   pdl_trigger();
-  pdl_wait();
   const uint32_t p = blockIdx.x * 256u + threadIdx.x;
   const uint32_t row = div_by(p, per_row), col = (p - row * per_row.d) * kPiece;
   const bool here = p < pieces && col < (uint32_t)dim;
-  float h[kPiece];
-  zero16(h);
+  pdl_wait();
+  Packed16 g = {}, u = {};
   if (here) {
-    float g[kPiece], u[kPiece];
-    load16(gate_up + row * ld + col, g);
-    load16(gate_up + row * ld + dim + col, u);
+    g = load16(gate_up + row * ld + col);
+    u = load16(gate_up + row * ld + dim + col);
+  }
+  float h[kPiece];
 #pragma unroll
-    for (int j = 0; j < kPiece; ++j) h[j] = g[j] / (1.0f + expf(-g[j])) * u[j];
+  for (int j = 0; j < 8; ++j) {
+    h[2 * j] = low(g.w[j]) * sigmoid(low(g.w[j])) * low(u.w[j]);
+    h[2 * j + 1] = high(g.w[j]) * sigmoid(high(g.w[j])) * high(u.w[j]);
   }
   const float s = block_inv_scale(lanes8_max(magnitude16(h)));
   if (here) {
@@ -195,7 +247,7 @@ __global__ void __launch_bounds__(256) silu_mul_blocks_kernel(const __nv_bfloat1
   }
 }
 
-static bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+static bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
 
 // What the four casts ask of a [rows, cols] result.
 static int check_rows(const char* what, int64_t rows, int64_t cols) {
@@ -216,7 +268,7 @@ static void launch_rmsnorm_blocks(cudaStream_t s, const void* x, const void* res
                                   int64_t rows, int cols, void* sum, void* q, float* inv) {
   launch_kernel(rmsnorm_blocks_kernel<NP, NT>, dim3((unsigned)rows), dim3(NT), 0, s, 1, static_cast<const __nv_bfloat16*>(x),
                 static_cast<const __nv_bfloat16*>(residual), static_cast<const __nv_bfloat16*>(weight), eps, cols,
-                (cols + 127) / 128, static_cast<uint4*>(sum), static_cast<uint8_t*>(q), inv);
+                (cols + 127) / 128, static_cast<__nv_bfloat16*>(sum), static_cast<uint8_t*>(q), inv);
 }
 
 }  // namespace xaxb
@@ -227,9 +279,9 @@ extern "C" {
 
 int xaxb_quantize_blocks(xaxb_ctx* ctx, void* stream, const void* x_bf16, int64_t rows, int64_t cols, int block_rows,
                          void* q_e4m3, float* inv_scale) {
-  if (!ctx || !x_bf16 || !q_e4m3 || !inv_scale || misaligned16(x_bf16) || misaligned16(q_e4m3) ||
+  if (!ctx || !x_bf16 || !q_e4m3 || !inv_scale || misaligned(x_bf16, 32) || misaligned(q_e4m3, 16) ||
       (block_rows != 1 && block_rows != 128)) {
-    set_last_error("quantize_blocks: x and q must be 16-byte aligned, block_rows 1 or 128");
+    set_last_error("quantize_blocks: x must be 32-byte aligned, q 16-byte aligned, block_rows 1 or 128");
     return XAXB_BAD_ARGUMENT;
   }
   if (int rc = check_rows("quantize_blocks", rows, cols)) return rc;
@@ -254,34 +306,37 @@ int xaxb_quantize_blocks(xaxb_ctx* ctx, void* stream, const void* x_bf16, int64_
 int xaxb_rmsnorm_blocks(xaxb_ctx* ctx, void* stream, const void* x_bf16, const void* residual_bf16, const void* weight_bf16,
                         float eps, int64_t rows, int64_t cols, void* sum_bf16, void* q_e4m3, float* inv_scale) {
   if (!ctx || !x_bf16 || !weight_bf16 || !q_e4m3 || !inv_scale || (residual_bf16 != nullptr) != (sum_bf16 != nullptr) ||
-      misaligned16(x_bf16) || misaligned16(residual_bf16) || misaligned16(weight_bf16) || misaligned16(sum_bf16) ||
-      misaligned16(q_e4m3)) {
-    set_last_error("rmsnorm_blocks: tensors must be 16-byte aligned; a sum goes with a residual");
+      misaligned(x_bf16, 32) || misaligned(residual_bf16, 32) || misaligned(weight_bf16, 32) || misaligned(sum_bf16, 32) ||
+      misaligned(q_e4m3, 16)) {
+    set_last_error("rmsnorm_blocks: bf16 tensors must be 32-byte aligned, q 16-byte aligned; a sum goes with a residual");
     return XAXB_BAD_ARGUMENT;
   }
   if (int rc = check_rows("rmsnorm_blocks", rows, cols)) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int pieces = (int)((cols + 127) / 128) * kBlockPieces;
-#define XAXB_NORM(NP, NT) \
-  launch_rmsnorm_blocks<NP, NT>(s, x_bf16, residual_bf16, weight_bf16, eps, rows, (int)cols, sum_bf16, q_e4m3, inv_scale)
-  if (pieces <= 128) XAXB_NORM(1, 128);
-  else if (pieces <= 256) XAXB_NORM(1, 256);
-  else if (pieces <= 512) XAXB_NORM(1, 512);
-  else if (pieces <= 1024) XAXB_NORM(2, 512);
-  else if (pieces <= 2048) XAXB_NORM(4, 512);
-  else {
+  if (pieces > 2048) {
     set_last_error("rmsnorm_blocks: rows of at most 32768 values, got %lld", (long long)cols);
     return XAXB_UNSUPPORTED;
   }
+  const bool many = rows >= 4 * reinterpret_cast<const Ctx*>(ctx)->num_sms;
+#define XAXB_NORM(NP, NT) \
+  launch_rmsnorm_blocks<NP, NT>(s, x_bf16, residual_bf16, weight_bf16, eps, rows, (int)cols, sum_bf16, q_e4m3, inv_scale)
+  if (pieces <= 128) XAXB_NORM(1, 128);
+  else if (pieces <= 256 && many) XAXB_NORM(2, 128);
+  else if (pieces <= 256) XAXB_NORM(1, 256);
+  else if (pieces <= 512 && many) XAXB_NORM(2, 256);
+  else if (pieces <= 512) XAXB_NORM(1, 512);
+  else if (pieces <= 1024) XAXB_NORM(2, 512);
+  else XAXB_NORM(4, 512);
 #undef XAXB_NORM
   return check_launch("rmsnorm_blocks_kernel");
 }
 
 int xaxb_silu_mul_blocks(xaxb_ctx* ctx, void* stream, const void* gate_up_bf16, int64_t ld, int64_t rows, int64_t dim,
                          void* q_e4m3, float* inv_scale) {
-  if (!ctx || !gate_up_bf16 || !q_e4m3 || !inv_scale || misaligned16(gate_up_bf16) || misaligned16(q_e4m3) || ld % 8 != 0 ||
+  if (!ctx || !gate_up_bf16 || !q_e4m3 || !inv_scale || misaligned(gate_up_bf16, 32) || misaligned(q_e4m3, 16) || ld % 16 != 0 ||
       ld < 2 * dim) {
-    set_last_error("silu_mul_blocks: gate_up and q must be 16-byte aligned, ld a multiple of 8 and at least twice the width");
+    set_last_error("silu_mul_blocks: gate_up must be 32-byte aligned, q 16-byte aligned, ld a multiple of 16 and at least twice the width");
     return XAXB_BAD_ARGUMENT;
   }
   if (int rc = check_rows("silu_mul_blocks", rows, dim)) return rc;

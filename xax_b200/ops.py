@@ -217,91 +217,110 @@ def dequantize_e5m2(q: torch.Tensor, scale: torch.Tensor, out_dtype=BF16) -> tor
 # ---------------------------------------------------------------------------------------
 # block-scaled e4m3: (q, inv_scale) with one float32 multiplier per 128 columns of a row, or per 128 x 128 square
 
+# Their kernels take a few microseconds, so the wrappers test everything a good call has in one expression and turn to the
+# helper that copies or refuses only where that fails.
+
 SCALE_BLOCK = 128
+F32 = torch.float32
 
 
 def _blocks(n: int) -> int:
     return -(-n // SCALE_BLOCK)
 
 
-def _req_blocks(what: str, t: torch.Tensor, dtype, name: str, dim: int = 2) -> torch.Tensor:
-    """_req for the block-scaled operators: also of rank ``dim``, and on the device whose stream the kernel goes to."""
+def _is_input(t: torch.Tensor, dtype, dim: int, device: int) -> bool:
+    return t.dtype is dtype and t.get_device() == device and t.dim() == dim and t.is_contiguous()
+
+
+def _block_input(what: str, t: torch.Tensor, dtype, name: str, dim: int = 2, align: int = 1) -> torch.Tensor:
+    """A contiguous tensor of the type, rank and alignment asked for, copied if need be, or the refusal."""
+    t = _req(t, dtype, name)
     if t.dim() != dim:
         raise ValueError(f"{what}: {name} must be {dim}-D, got {tuple(t.shape)}")
-    t = _req(t, dtype, name)
     if t.get_device() != torch.cuda.current_device():
         raise ValueError(f"{what}: {name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-    return t
+    return t.clone() if t.data_ptr() % align else t
 
 
-def _req_rows(what: str, t: torch.Tensor, dtype, name: str) -> None:
-    """The same for an operand that is read or written through its row stride, with nothing copied."""
+def _check_rows(what: str, t: torch.Tensor, dtype, name: str, shape=None) -> None:
+    """Refuses a matrix that the kernel could not read or write through its row stride."""
     if not t.is_cuda or t.dtype != dtype or t.dim() != 2:
         raise ValueError(f"{what}: {name} must be a 2-D {dtype} CUDA tensor (there is no CPU fallback)")
-    if t.stride(1) != 1 and t.shape[1] > 1:
-        raise ValueError(f"{what}: the rows of {name} must be contiguous")
     if t.get_device() != torch.cuda.current_device():
         raise ValueError(f"{what}: {name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        raise ValueError(f"{what}: the rows of {name} must be contiguous")
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{what}: {name} must be {list(shape)}, got {tuple(t.shape)}")
 
 
-def _cast_outputs(x: torch.Tensor, rows: int, cols: int, block_rows: int = 1):
-    return (x.new_empty((rows, cols), dtype=E4M3),
-            x.new_empty((-(-rows // block_rows), -(-cols // SCALE_BLOCK)), dtype=torch.float32))
+def _device_of(t: torch.Tensor) -> int:
+    """The current device if ``t`` is on it, else -2 (on which no tensor is, so that the helpers get to refuse it)."""
+    return t.get_device() if t.is_cuda and t.get_device() == torch.cuda.current_device() else -2
 
 
 def quantize_blocks(x: torch.Tensor, block_rows: int = 1):
     """x[rows, cols] bf16 -> (q e4m3 [rows, cols], inv_scale f32 [rows, ceil(cols / 128)]): the cast with one scale per
     row and 128 columns, or with ``block_rows = 128`` per 128 x 128 square (weights; inv_scale then has
     ceil(rows / 128) rows).  x ~ q * inv_scale.  cols must be a multiple of 16."""
-    x = _req_blocks("quantize_blocks", x, BF16, "x")
-    if block_rows not in (1, SCALE_BLOCK):
+    dev = _device_of(x)
+    if not _is_input(x, BF16, 2, dev) or x.data_ptr() % 32:
+        x = _block_input("quantize_blocks", x, BF16, "x", align=32)
+        dev = x.get_device()
+    if block_rows != 1 and block_rows != SCALE_BLOCK:
         raise ValueError(f"quantize_blocks: block_rows must be 1 or {SCALE_BLOCK}, got {block_rows}")
     rows, cols = x.shape
-    q, inv = _cast_outputs(x, rows, cols, block_rows)
+    q = torch.empty_like(x, dtype=E4M3)
+    inv = x.new_empty((-(-rows // block_rows), -(-cols // SCALE_BLOCK)), dtype=F32)
     if rows == 0:
         return q, inv
-    ctx, st, lib = _c()
-    check(lib.xaxb_quantize_blocks(ctx, st, ptr(x), rows, cols, block_rows, ptr(q), ptr(inv)), "quantize_blocks")
+    ctx, st, lib = _lib.call_state(dev)
+    check(lib.xaxb_quantize_blocks(ctx, st, x.data_ptr(), rows, cols, block_rows, q.data_ptr(), inv.data_ptr()),
+          "quantize_blocks")
     return q, inv
 
 
 def gemm_fp8_blocks(a_q, b_q, a_inv, b_inv, bias=None, residual=None, out=None):
     """Product of block-scaled operands: activations (a_q e4m3 [M, K], a_inv f32 [M, ceil(K / 128)]) and weights
     (b_q e4m3 [N, K], b_inv f32 [ceil(N / 128), ceil(K / 128)]) -> bf16 [M, N] = A @ B.T + bias + residual.  K must be
-    a multiple of 16 and N of 8."""
+    a multiple of 16 and N of 8.  ``out`` may be ``residual``; otherwise it must not overlap an operand."""
     what = "gemm_fp8_blocks"
-    _req_rows(what, a_q, E4M3, "a_q")
-    _req_rows(what, b_q, E4M3, "b_q")
+    dev = _device_of(a_q)
+    if not (_is_input(a_q, E4M3, 2, dev) and _is_input(b_q, E4M3, 2, dev)):  # (contiguous, or rows apart: both will do)
+        _check_rows(what, a_q, E4M3, "a_q")
+        _check_rows(what, b_q, E4M3, "b_q")
+        dev = a_q.get_device()
     (M, K), (N, Kb) = a_q.shape, b_q.shape
     if K != Kb:
         raise ValueError(f"{what}: inner dimensions differ ({K} vs {Kb})")
-    a_inv = _req_blocks(what, a_inv, torch.float32, "a_inv")
-    b_inv = _req_blocks(what, b_inv, torch.float32, "b_inv")
-    if a_inv.shape != (M, _blocks(K)) or b_inv.shape != (_blocks(N), _blocks(K)):
+    if not (_is_input(a_inv, F32, 2, dev) and _is_input(b_inv, F32, 2, dev)):
+        a_inv, b_inv = _block_input(what, a_inv, F32, "a_inv"), _block_input(what, b_inv, F32, "b_inv")
+    blocks = -(-K // SCALE_BLOCK)
+    if a_inv.shape != (M, blocks) or b_inv.shape != (-(-N // SCALE_BLOCK), blocks):
         raise ValueError(f"{what}: a_inv {tuple(a_inv.shape)} and b_inv {tuple(b_inv.shape)} must be "
-                         f"({M}, {_blocks(K)}) and ({_blocks(N)}, {_blocks(K)})")
+                         f"({M}, {blocks}) and ({_blocks(N)}, {blocks})")
+    bias_ptr = res_ptr = None
+    ldr = 0
     if bias is not None:
-        bias = _req_blocks(what, bias, BF16, "bias", 1)
+        if not _is_input(bias, BF16, 1, dev):
+            bias = _block_input(what, bias, BF16, "bias", 1)
         if bias.shape[0] != N:
             raise ValueError(f"{what}: bias must be [{N}], got {tuple(bias.shape)}")
+        bias_ptr = bias.data_ptr()
+    if residual is not None:
+        if residual.shape != (M, N) or not _is_input(residual, BF16, 2, dev):
+            _check_rows(what, residual, BF16, "residual", (M, N))
+        res_ptr, ldr = residual.data_ptr(), residual.stride(0) if M > 1 else N
     if out is None:
         out = a_q.new_empty((M, N), dtype=BF16)
     else:
-        _req_rows(what, out, BF16, "out")
-        if out.shape != (M, N):
-            raise ValueError(f"{what}: out must be [{M}, {N}], got {tuple(out.shape)}")
-    ldr = 0
-    if residual is not None:
-        _req_rows(what, residual, BF16, "residual")
-        if residual.shape != (M, N):
-            raise ValueError(f"{what}: residual must be [{M}, {N}], got {tuple(residual.shape)}")
-        ldr = residual.stride(0) if M > 1 else N
+        _check_rows(what, out, BF16, "out", (M, N))
     if M == 0:
         return out
     lda, ldo = (a_q.stride(0), out.stride(0)) if M > 1 else (K, N)  # the stride of a single row may be anything
-    ctx, st, lib = _c()
-    check(lib.xaxb_gemm_fp8_blocks(ctx, st, ptr(a_q), lda, ptr(a_inv), ptr(b_q), b_q.stride(0), ptr(b_inv), M, N, K, ptr(bias),
-                                   ptr(residual), ldr, ptr(out), ldo), what)
+    ctx, st, lib = _lib.call_state(dev)
+    check(lib.xaxb_gemm_fp8_blocks(ctx, st, a_q.data_ptr(), lda, a_inv.data_ptr(), b_q.data_ptr(), b_q.stride(0),
+                                   b_inv.data_ptr(), M, N, K, bias_ptr, res_ptr, ldr, out.data_ptr(), ldo), what)
     return out
 
 
@@ -309,38 +328,48 @@ def rmsnorm_blocks(x, weight, eps, *, residual=None):
     """RMSNorm of x (+ residual) [rows, cols] bf16 followed by the cast of quantize_blocks, in float32 from the inputs to
     the 8 bits.  Returns (x + residual as bf16, or None without a residual; q; inv_scale)."""
     what = "rmsnorm_blocks"
-    x = _req_blocks(what, x, BF16, "x")
+    dev = _device_of(x)
+    if not (_is_input(x, BF16, 2, dev) and _is_input(weight, BF16, 1, dev)) or (x.data_ptr() | weight.data_ptr()) % 32:
+        x, weight = _block_input(what, x, BF16, "x", align=32), _block_input(what, weight, BF16, "weight", 1, 32)
+        dev = x.get_device()
     rows, cols = x.shape
-    weight = _req_blocks(what, weight, BF16, "weight", 1)
     if weight.shape[0] != cols:
         raise ValueError(f"{what}: weight must be [{cols}], got {tuple(weight.shape)}")
-    total = None
+    total = total_ptr = res_ptr = None
     if residual is not None:
-        residual = _req_blocks(what, residual, BF16, "residual")
+        if not _is_input(residual, BF16, 2, dev) or residual.data_ptr() % 32:
+            residual = _block_input(what, residual, BF16, "residual", align=32)
         if residual.shape != x.shape:
             raise ValueError(f"{what}: residual {tuple(residual.shape)} must have x's shape {tuple(x.shape)}")
         total = torch.empty_like(x)
-    q, inv = _cast_outputs(x, rows, cols)
+        res_ptr, total_ptr = residual.data_ptr(), total.data_ptr()
+    q = torch.empty_like(x, dtype=E4M3)
+    inv = x.new_empty((rows, -(-cols // SCALE_BLOCK)), dtype=F32)
     if rows == 0:
         return total, q, inv
-    ctx, st, lib = _c()
-    check(lib.xaxb_rmsnorm_blocks(ctx, st, ptr(x), ptr(residual), ptr(weight), float(eps), rows, cols, ptr(total), ptr(q),
-                                  ptr(inv)), what)
+    ctx, st, lib = _lib.call_state(dev)
+    check(lib.xaxb_rmsnorm_blocks(ctx, st, x.data_ptr(), res_ptr, weight.data_ptr(), eps, rows, cols, total_ptr, q.data_ptr(),
+                                  inv.data_ptr()), what)
     return total, q, inv
 
 
 def silu_mul_blocks(gate_up, dim: int):
     """silu(gate) * up of gate_up [rows, 2*dim] bf16 (gate | up), in float32, followed by the cast of quantize_blocks.
     Returns (q e4m3 [rows, dim], inv_scale f32 [rows, ceil(dim / 128)])."""
-    gate_up = _req_blocks("silu_mul_blocks", gate_up, BF16, "gate_up")
+    dev = _device_of(gate_up)
+    if not _is_input(gate_up, BF16, 2, dev) or gate_up.data_ptr() % 32:
+        gate_up = _block_input("silu_mul_blocks", gate_up, BF16, "gate_up", align=32)
+        dev = gate_up.get_device()
     rows, ld = gate_up.shape
     if dim <= 0 or ld != 2 * dim:
         raise ValueError(f"silu_mul_blocks: gate_up must be [rows, 2 * {dim}], got {tuple(gate_up.shape)}")
-    q, inv = _cast_outputs(gate_up, rows, dim)
+    q = gate_up.new_empty((rows, dim), dtype=E4M3)
+    inv = gate_up.new_empty((rows, -(-dim // SCALE_BLOCK)), dtype=F32)
     if rows == 0:
         return q, inv
-    ctx, st, lib = _c()
-    check(lib.xaxb_silu_mul_blocks(ctx, st, ptr(gate_up), ld, rows, dim, ptr(q), ptr(inv)), "silu_mul_blocks")
+    ctx, st, lib = _lib.call_state(dev)
+    check(lib.xaxb_silu_mul_blocks(ctx, st, gate_up.data_ptr(), ld, rows, dim, q.data_ptr(), inv.data_ptr()),
+          "silu_mul_blocks")
     return q, inv
 
 
