@@ -208,42 +208,57 @@ __global__ void __launch_bounds__(NT) rmsnorm_blocks_kernel(const __nv_bfloat16*
 
 // ---- silu(gate) * up, gate and up the two halves of a row of the fused gate | up product.
 
-// 1 / (1 + e^-g) to a few units: e^-g = 2^h (1 + l ln 2) with h + l = -g log2 e to twice the precision, from the
-// approximate exponential and reciprocal (2^-22 each).  Below -87 the exponential nears the end of its range and the
-// result is 0 in float32 to every purpose; NaN passes through the product with g.
-__device__ __forceinline__ float sigmoid(float g) {
-  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-  const float x = -fmaxf(g, -87.0f), h = x * kLog2e, l = fmaf(x, kLog2e, -h);
+// 1 / (1 + e^x) to a few units: e^x = 2^h (1 + l) with h = x log2 e rounded and l = x - h ln 2, from the approximate
+// exponential and reciprocal (2^-22 each).  x is kept from -88 up, where e^x is nothing beside 1, and h up to 127, past
+// which the result is below the smallest normal float; NaN comes back in the product with the gate.
+__device__ __forceinline__ float one_over_one_plus_exp(float x) {
+  x = fmaxf(x, -88.0f);
+  const float h = fminf(x * 1.4426950408889634f, 127.0f);
   float e, r;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(h));
-  e = fmaf(e, l * kLn2, e);
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return g < -87.0f ? 0.0f : r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(h));
+  e = fmaf(e, fmaf(h, -0.6931471805599453f, x), e);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return r;
 }
 
+__device__ __forceinline__ float silu_mul(float g, float u) { return g * one_over_one_plus_exp(-g) * u; }
+
+// A grid of resident CTAs walks the pieces; the next piece's loads are under way while one is computed (an exponential, a
+// reciprocal and a dozen more instructions per value take about as long as its bytes: 27.5 us without, see the launcher).
 __global__ void __launch_bounds__(256) silu_mul_blocks_kernel(const __nv_bfloat16* __restrict__ gate_up, int64_t ld,
                                                               uint32_t pieces, FastDiv per_row, int dim,
                                                               uint8_t* __restrict__ q, float* __restrict__ inv) {
   pdl_trigger();
-  const uint32_t p = blockIdx.x * 256u + threadIdx.x;
-  const uint32_t row = div_by(p, per_row), col = (p - row * per_row.d) * kPiece;
-  const bool here = p < pieces && col < (uint32_t)dim;
+  const uint32_t step = gridDim.x * 256u;
+  Packed16 g, u;
+  auto ask = [&](uint32_t p) {
+    const uint32_t row = div_by(p, per_row), col = (p - row * per_row.d) * kPiece;
+    g = {}, u = {};
+    if (p < pieces && col < (uint32_t)dim) {
+      g = load16(gate_up + row * ld + col);
+      u = load16(gate_up + row * ld + dim + col);
+    }
+  };
+  uint32_t p = blockIdx.x * 256u + threadIdx.x;
   pdl_wait();
-  Packed16 g = {}, u = {};
-  if (here) {
-    g = load16(gate_up + row * ld + col);
-    u = load16(gate_up + row * ld + dim + col);
-  }
-  float h[kPiece];
+  ask(p);
+  // (pieces is a multiple of 8 and CTAs start at multiples of 256: the eight lanes of a block stay together.  p cannot
+  // wrap: pieces < 2^31 and step < 2^20.)
+  for (uint32_t base = blockIdx.x * 256u; base < pieces; base += step, p += step) {
+    const Packed16 gn = g, un = u;
+    if (base + step < pieces) ask(p + step);
+    float h[kPiece];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    h[2 * j] = low(g.w[j]) * sigmoid(low(g.w[j])) * low(u.w[j]);
-    h[2 * j + 1] = high(g.w[j]) * sigmoid(high(g.w[j])) * high(u.w[j]);
-  }
-  const float s = block_inv_scale(lanes8_max(magnitude16(h)));
-  if (here) {
-    *reinterpret_cast<uint4*>(q + (int64_t)row * dim + col) = cast16(h, 1.0f / s);
-    if (p % kBlockPieces == 0) inv[p / kBlockPieces] = s;
+    for (int j = 0; j < 8; ++j) {
+      h[2 * j] = silu_mul(low(gn.w[j]), low(un.w[j]));
+      h[2 * j + 1] = silu_mul(high(gn.w[j]), high(un.w[j]));
+    }
+    const float s = block_inv_scale(lanes8_max(magnitude16(h)));
+    const uint32_t row = div_by(p, per_row), col = (p - row * per_row.d) * kPiece;
+    if (p < pieces && col < (uint32_t)dim) {
+      *reinterpret_cast<uint4*>(q + (int64_t)row * dim + col) = cast16(h, 1.0f / s);
+      if (p % kBlockPieces == 0) inv[p / kBlockPieces] = s;
+    }
   }
 }
 
@@ -341,7 +356,8 @@ int xaxb_silu_mul_blocks(xaxb_ctx* ctx, void* stream, const void* gate_up_bf16, 
   }
   if (int rc = check_rows("silu_mul_blocks", rows, dim)) return rc;
   const uint32_t per_row = (uint32_t)((dim + 127) / 128 * kBlockPieces), pieces = (uint32_t)(rows * per_row);
-  launch_kernel(silu_mul_blocks_kernel, dim3((pieces + 255) / 256), dim3(256), 0, static_cast<cudaStream_t>(stream), 1,
+  const unsigned ctas = (pieces + 255) / 256, resident = 4u * reinterpret_cast<const Ctx*>(ctx)->num_sms;
+  launch_kernel(silu_mul_blocks_kernel, dim3(ctas < resident ? ctas : resident), dim3(256), 0, static_cast<cudaStream_t>(stream), 1,
                 static_cast<const __nv_bfloat16*>(gate_up_bf16), ld, pieces, fast_div(per_row), (int)dim,
                 static_cast<uint8_t*>(q_e4m3), inv_scale);
   return check_launch("silu_mul_blocks_kernel");
