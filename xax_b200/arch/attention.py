@@ -25,7 +25,7 @@ from typing import Literal, NotRequired, TypedDict
 import torch
 
 from .. import ops
-from ..nn.fp8 import Fp8Linear, Fp8Scales, init_fp8_scales
+from ..nn.fp8 import Fp8BlockLinear, Fp8Linear, Fp8Scales, StackedBlockLinears, init_fp8_scales
 from ..nn.lora import LoRALinear
 
 BF16 = torch.bfloat16
@@ -91,6 +91,8 @@ def apply_linear(x: torch.Tensor, linear, *, residual: torch.Tensor | None = Non
             res2 = None if residual is None else residual.reshape(B * T, -1)
             return linear.forward_quantized(xq, x_inv, res2).reshape(B, T, -1)
         return linear(x, residual=residual)[0]
+    if isinstance(linear, Fp8BlockLinear):  # one scale per token and 128 features, batched or not
+        return linear(x, residual=residual)
     if isinstance(linear, Linear):
         x2 = x.reshape(-1, x.shape[-1]).to(BF16).contiguous()
         res2 = None if residual is None else residual.reshape(-1, linear.out_features)
@@ -143,21 +145,24 @@ class RMSNorm:
 
 class SwiGLU:
     """xax/arch/attention.py:101-147: down(silu(gate(x)) * up(x)).  ``build`` uses plain
-    linears like the reference (:138-140); pass ``use_fp8=True`` (an extension) or swap
-    Fp8Linear instances into ``gate`` / ``up`` / ``down`` for the FP8 MLP."""
+    linears like the reference (:138-140); pass ``use_fp8=True`` or ``fp8_blocks=True`` (extensions) or
+    swap Fp8Linear / Fp8BlockLinear instances into ``gate`` / ``up`` / ``down`` for the FP8 MLP."""
 
     def __init__(self, gate, up, down):
         self.gate, self.up, self.down = gate, up, down
         self._fused = None
         self._fused_key = None
+        self._stack = None
 
     @classmethod
     def build(cls, embed_dim: int, hidden_dim: int | None = None, *, key=None, use_bias: bool = False,
-              use_fp8: bool = False, device=None) -> "SwiGLU":
+              use_fp8: bool = False, device=None, fp8_blocks: bool = False) -> "SwiGLU":
         if hidden_dim is None:
             hidden_dim = embed_dim * 4
         seed = int(key or 0) if not isinstance(key, torch.Generator) else int(key.initial_seed())
-        if use_fp8:
+        if fp8_blocks:
+            mk = lambda i, o, k: Fp8BlockLinear(i, o, key=k, use_bias=use_bias, device=device)  # noqa: E731
+        elif use_fp8:
             mk = lambda i, o, k: Fp8Linear(i, o, key=k, use_bias=use_bias, device=device)  # noqa: E731
         else:
             mk = lambda i, o, k: Linear(i, o, use_bias=use_bias, key=k, device=device)  # noqa: E731
@@ -166,6 +171,14 @@ class SwiGLU:
 
     def is_fp8(self) -> bool:
         return all(isinstance(m, Fp8Linear) and m.use_fp8 for m in (self.gate, self.up, self.down))
+
+    def is_fp8_blocks(self) -> bool:
+        return all(isinstance(m, Fp8BlockLinear) for m in (self.gate, self.up, self.down))
+
+    def _gate_up_stack(self) -> StackedBlockLinears:
+        if self._stack is None or self._stack.layers != (self.gate, self.up):
+            self._stack = StackedBlockLinears((self.gate, self.up))
+        return self._stack
 
     def fused_gate_up(self):
         """gate | up weights stacked into one [2F, H] operand so one GEMM reads x once."""
@@ -197,7 +210,16 @@ class SwiGLU:
 
     def forward_tokens(self, y: torch.Tensor, B: int, T: int, *, residual=None, y_q=None) -> torch.Tensor:
         """y: normalised activations [B*T, H].  One activation scale per sequence (T rows).
-        ``y_q`` = (q, inv_scale) when the preceding RMSNorm already cast y."""
+        ``y_q`` = (q, inv_scale) when the preceding RMSNorm already cast y (block-scaled layers: by
+        rmsnorm_blocks; y is then not read)."""
+        if self.is_fp8_blocks():
+            q, inv = ops.quantize_blocks(y) if y_q is None else y_q
+            hq, h_inv = ops.silu_mul_blocks(self._gate_up_stack()(q, inv), self.gate.out_features)
+            return self.down.forward_quantized(hq, h_inv, residual)
+        if any(isinstance(m, Fp8BlockLinear) for m in (self.gate, self.up)):  # layers of several kinds: one by one
+            gu = torch.cat([apply_linear(y, self.gate), apply_linear(y, self.up)], dim=1)
+            h, _ = ops.silu_mul(gu, self.gate.out_features)
+            return apply_linear(h, self.down, residual=residual)
         wq, col, bias = self.fused_gate_up()
         F = self.gate.out_features
         if self.is_fp8():
@@ -242,8 +264,12 @@ class TransformerBlockCache(TypedDict):
     self_attn_fp8: NotRequired[Fp8ScalesCache]
 
 
-def _make_linear(in_features, out_features, key, use_bias=True, use_fp8=False, compute_dtype=BF16, device=None):
-    """xax/arch/attention.py:212-241 (an FP8 layer always gets a bias, like the reference)."""
+def _make_linear(in_features, out_features, key, use_bias=True, use_fp8=False, compute_dtype=BF16, device=None,
+                 fp8_blocks=False):
+    """xax/arch/attention.py:212-241 (an FP8 layer always gets a bias, like the reference; a block-scaled one, which the
+    reference has not, as asked)."""
+    if fp8_blocks:
+        return Fp8BlockLinear(in_features, out_features, key=key, use_bias=use_bias, device=device)
     if use_fp8:
         return Fp8Linear(in_features, out_features, key=key, use_fp8=True, compute_dtype=compute_dtype, device=device)
     return Linear(in_features, out_features, use_bias=use_bias, key=key, device=device)
@@ -352,6 +378,7 @@ class SelfAttentionBlock:
         self.causal, self.local_window_size, self.use_fp8 = causal, local_window_size, use_fp8
         self._fused = None
         self._fused_key = None
+        self._stack = None
 
     @classmethod
     def build(cls, embed_dim: int, num_heads: int, *, key=None, num_kv_heads: int | None = None,
@@ -361,14 +388,14 @@ class SelfAttentionBlock:
               rotary_original_max_position_embeddings: int | None = None, rotary_beta_slow: float = 1.0,
               rotary_beta_fast: float = 32.0, use_qk_norm: bool = False, qk_norm_eps: float = 1e-6,
               use_attention_sinks: bool = False, use_fp8: bool = False, compute_dtype=BF16,
-              device=None) -> "SelfAttentionBlock":
+              device=None, fp8_blocks: bool = False) -> "SelfAttentionBlock":
         sinks = torch.zeros((num_heads,), dtype=torch.float32, device=device) if use_attention_sinks else None  # :652-654
         kv = num_kv_heads if num_kv_heads is not None else num_heads
         hd = head_dim if head_dim is not None else embed_dim // num_heads
         assert num_heads % kv == 0, "num_heads must be divisible by num_kv_heads"  # :620
         seed = int(key or 0) if not isinstance(key, torch.Generator) else int(key.initial_seed())
         qd, kd = num_heads * hd, kv * hd
-        mk = lambda i, o, k: _make_linear(i, o, k, use_bias, use_fp8, compute_dtype, device)  # noqa: E731
+        mk = lambda i, o, k: _make_linear(i, o, k, use_bias, use_fp8, compute_dtype, device, fp8_blocks)  # noqa: E731
         rope = RotaryEmbedding.build(hd, rotary_base, rotary_style, rotary_factor,
                                      rotary_original_max_position_embeddings, rotary_beta_slow,
                                      rotary_beta_fast) if use_rotary_embeddings else None
@@ -385,6 +412,15 @@ class SelfAttentionBlock:
 
     def _is_fp8(self) -> bool:
         return all(isinstance(m, Fp8Linear) and m.use_fp8 for m in (self.q_proj, self.k_proj, self.v_proj))
+
+    def is_fp8_blocks(self) -> bool:
+        return all(isinstance(m, Fp8BlockLinear) for m in (self.q_proj, self.k_proj, self.v_proj))
+
+    def _qkv_stack(self) -> StackedBlockLinears:
+        projs = (self.q_proj, self.k_proj, self.v_proj)
+        if self._stack is None or self._stack.layers != projs:
+            self._stack = StackedBlockLinears(projs)
+        return self._stack
 
     def fused_qkv(self):
         """q | k | v weights stacked into one [(Hq + 2 Hkv) D, H] operand; per-column
@@ -532,14 +568,22 @@ class SelfAttentionBlock:
         elif not donate:
             cache = {"k": cache["k"].clone(), "v": cache["v"].clone(), "position": cache["position"].clone()}
         max_len = cache["k"].shape[1]
-        wq, col, bias = self.fused_qkv()
-        if self._is_fp8():  # per-token activation scales (vmapped layer, :279)
+        blocks = self.is_fp8_blocks()
+        projs = (self.q_proj, self.k_proj, self.v_proj)
+        if blocks:  # block-scaled layers: one scale per token and 128 features
+            q, inv = ops.quantize_blocks(y.to(BF16)) if y_q is None else y_q
+            qkv = self._qkv_stack()(q, inv)
+        elif any(isinstance(m, Fp8BlockLinear) for m in projs):  # layers of several kinds: one by one
+            qkv = torch.cat([apply_linear(y, m) for m in projs], dim=1)
+        elif self._is_fp8():  # per-token activation scales (vmapped layer, :279)
+            wq, col, bias = self.fused_qkv()
             if y_q is None:
                 q, _, inv, _ = ops.quantize_current(y.to(BF16).contiguous(), 1)
             else:
                 q, inv = y_q
             qkv = ops.gemm_fp8(q, wq, inv, col, bias)
         else:
+            wq, col, bias = self.fused_qkv()
             qkv = ops.gemm_bf16(y.to(BF16).contiguous(), wq, None, None, bias)
         if self.rotary_emb is None:
             raise ValueError("the attention kernels expect rotary embeddings (as the LLM builds them)")
@@ -725,11 +769,12 @@ class TransformerBlock:
               rotary_beta_fast: float = 32.0, use_qk_norm: bool = False, qk_norm_eps: float = 1e-6,
               use_attention_sinks: bool = False, norm_type: str = "layernorm", norm_eps: float = 1e-6,
               feedforward_type: str = "mlp", use_fp8: bool = False, compute_dtype=BF16, fp8_mlp: bool | None = None,
-              device=None) -> "TransformerBlock":
+              device=None, fp8_blocks: bool = False) -> "TransformerBlock":
         """Same keyword arguments as the reference.  ``norm_type`` must be "rmsnorm" and
         ``feedforward_type`` "swiglu" (the LLM path).  Like the reference, ``use_fp8`` makes the
         four attention projections FP8 and leaves the SwiGLU on plain linears (:1354-1355);
-        ``fp8_mlp=True`` (an extension) builds the SwiGLU from Fp8Linear too."""
+        ``fp8_mlp=True`` (an extension) builds the SwiGLU from Fp8Linear too, ``fp8_blocks=True``
+        (another) all of self-attention and SwiGLU from Fp8BlockLinear."""
         if norm_type != "rmsnorm" or feedforward_type != "swiglu":
             raise ValueError("only norm_type='rmsnorm' with feedforward_type='swiglu' is on the path this library covers")
         seed = int(key or 0) if not isinstance(key, torch.Generator) else int(key.initial_seed())
@@ -741,8 +786,8 @@ class TransformerBlock:
             rotary_original_max_position_embeddings=rotary_original_max_position_embeddings,
             rotary_beta_slow=rotary_beta_slow, rotary_beta_fast=rotary_beta_fast, use_qk_norm=use_qk_norm,
             qk_norm_eps=qk_norm_eps, use_attention_sinks=use_attention_sinks, use_fp8=use_fp8,
-            compute_dtype=compute_dtype, device=device)
-        ff = SwiGLU.build(embed_dim, ff_dim, key=seed * 3 + 2, use_fp8=bool(fp8_mlp), device=device)
+            compute_dtype=compute_dtype, device=device, fp8_blocks=fp8_blocks)
+        ff = SwiGLU.build(embed_dim, ff_dim, key=seed * 3 + 2, use_fp8=bool(fp8_mlp), device=device, fp8_blocks=fp8_blocks)
         cross = cross_norm = None
         if cross_attention:  # :1312-1322
             cross = CrossAttentionBlock.build(embed_dim, num_heads, key=seed * 3 + 3,
@@ -829,6 +874,14 @@ class TransformerBlock:
         (+x) -> RMSNorm(+cast / amax) -> gate|up GEMM -> SiLU*up(+cast / amax) -> down GEMM (+x)."""
         attn, ff = self.self_attn, self.feed_forward
         wn = self.attn_norm.weight_bf16()
+        if attn.is_fp8_blocks() and ff.is_fp8_blocks():
+            # block-scaled layers: RMSNorm + cast -> QKV product -> RoPE + cache append -> attention -> cast -> out-proj
+            # product -> residual + RMSNorm + cast -> gate|up product -> SiLU*up + cast -> down product (+x)
+            _, q, inv = ops.rmsnorm_blocks(x, wn, self.attn_norm.eps)
+            o, new_cache = attn.forward_tokens(x, B, T, cache=cache, donate=donate, y_q=(q, inv), workspace=workspace,
+                                               advance=advance)
+            x1, q, inv = ops.rmsnorm_blocks(o, self.mlp_norm.weight_bf16(), self.mlp_norm.eps, residual=x)
+            return ff.forward_tokens(x1, B, T, residual=x1, y_q=(q, inv)), new_cache
         if attn._is_fp8():
             _, yq = ops.rmsnorm(x, wn, self.attn_norm.eps, want_y=False, quantize=True)
             x1, new_cache = attn.forward_tokens(x, B, T, cache=cache, donate=donate, y_q=(yq[0], yq[2]), residual=x,

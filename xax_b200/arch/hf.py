@@ -7,7 +7,9 @@ path).  Names, fall-backs and placement follow the reference: ``embed_tokens`` /
 ``post_attention_layernorm``, ``norm`` / ``ln_f``, each with or without the ``model.`` prefix; a
 checkpoint without ``lm_head.weight`` ties the head to the embedding.  Under tensor parallelism every
 rank keeps its slice per get_model_parallel_sharding_spec.  Weights are stored as bf16; the FP8 layers
-quantise them to e4m3 once, on first use.
+quantise them to e4m3 once, on first use.  Block-quantised checkpoints (e4m3 ``*.weight`` with float32
+``*.weight_scale_inv``, one multiplier per 128 x 128 square, announced by ``quantization_config`` /
+``weight_block_size``) load into Fp8BlockLinear layers as they are, and into other layers dequantised.
 """
 
 from __future__ import annotations
@@ -17,7 +19,7 @@ import os
 
 import torch
 
-from ..nn.fp8 import Fp8Linear
+from ..nn.fp8 import Fp8BlockLinear, Fp8Linear
 from .attention import Embedding, Linear, RMSNorm, RotaryEmbedding, SelfAttentionBlock, SwiGLU, TransformerBlock
 from .llm import LLM, LLMConfig, tie_embedding_and_head, tp_shard_dim
 
@@ -126,6 +128,25 @@ def _get_bias(state: dict, *names: str):
     return None
 
 
+def _block_quantised(cfg: dict) -> bool:
+    """Whether config.json announces block-scaled e4m3 weights; refuses squares of another size."""
+    qc = cfg.get("quantization_config")
+    size = qc.get("weight_block_size") if isinstance(qc, dict) else None
+    if size is None:
+        return False
+    if list(size) != [128, 128]:
+        raise ValueError(f"weight_block_size {list(size)}: block-scaled weights have a scale per 128 x 128 square here")
+    return True
+
+
+def _dequantise_blocks(name: str, w: torch.Tensor, inv: torch.Tensor) -> torch.Tensor:
+    """A block-quantised weight as bf16, on the host, for layers that scale differently."""
+    if tuple(inv.shape) != (-(-w.shape[0] // 128), -(-w.shape[1] // 128)):
+        raise ValueError(f"{name}: {tuple(inv.shape)} multipliers do not fit a weight {tuple(w.shape)} in 128 x 128 squares")
+    full = inv.float().repeat_interleave(128, 0)[:w.shape[0]].repeat_interleave(128, 1)[:, :w.shape[1]]
+    return (w.float() * full).to(BF16)
+
+
 def load_hf_weights_into_llm(model: LLM, repo_id: str | dict, revision: str | None = None, dtype=None) -> LLM:
     """xax/arch/llm.py:1191-1416.  ``repo_id`` is a local checkpoint directory (or an already loaded
     ``{name: tensor}`` dict); ``model`` supplies the structure (layer types, FP8 or not, tensor-parallel
@@ -150,7 +171,17 @@ def load_hf_weights_into_llm(model: LLM, repo_id: str | dict, revision: str | No
             arr = arr.narrow(dim, rank * n, n)
         return arr.to(device=dev, dtype=BF16).contiguous()
 
-    def map_linear(layer, w: torch.Tensor, b, weight_name: str):
+    def map_linear(layer, w: torch.Tensor, b, weight_name: str, inv=None):
+        if w.dtype == torch.float8_e4m3fn and inv is None:
+            raise KeyError(f"{weight_name}: e4m3 weight without weight_scale_inv in the checkpoint")
+        if isinstance(layer, Fp8BlockLinear):  # (never sharded, see LLM.build)
+            b_dev = None if b is None else place(b, weight_name + ".bias")
+            if w.dtype != torch.float8_e4m3fn:
+                w = place(w if w.shape == layer.weight.shape else w.t(), weight_name)
+                return Fp8BlockLinear(layer.in_features, layer.out_features, weight=w, bias=b_dev)
+            return Fp8BlockLinear(layer.in_features, layer.out_features, weight=w.to(dev), weight_inv=inv.to(dev), bias=b_dev)
+        if inv is not None:
+            w = _dequantise_blocks(weight_name, w, inv)
         full = list(layer.weight.shape)
         dim = tp_shard_dim(weight_name, 2)
         if size > 1 and dim is not None:
@@ -183,7 +214,8 @@ def load_hf_weights_into_llm(model: LLM, repo_id: str | dict, revision: str | No
 
         def proj(layer, prefix, name, tp_name):
             return map_linear(layer, _get_weight(state, *both(prefix, f"{name}.weight")),
-                              _get_bias(state, *both(prefix, f"{name}.bias")), tp_name)
+                              _get_bias(state, *both(prefix, f"{name}.bias")), tp_name,
+                              _get_bias(state, *both(prefix, f"{name}.weight_scale_inv")))
 
         attn = SelfAttentionBlock(
             proj(a.q_proj, sa, "q_proj", "q_proj"), proj(a.k_proj, sa, "k_proj", "k_proj"),
@@ -199,9 +231,12 @@ def load_hf_weights_into_llm(model: LLM, repo_id: str | dict, revision: str | No
                                        num_heads=a.num_heads, head_dim=a.head_dim, causal=a.causal, use_fp8=False))
     final = _get_bias(state, "norm.weight", "model.norm.weight", "ln_f.weight")
     norm = model.norm if final is None else RMSNorm(final.to(device=dev, dtype=BF16).contiguous(), model.norm.eps)
-    head_keys = [k for k in state if "lm_head.weight" in k]
+    head_keys = [k for k in state if k.endswith("lm_head.weight")]
     if head_keys:
-        hw = state[head_keys[0]].to(device=dev, dtype=BF16).contiguous()
+        hw = state[head_keys[0]]
+        if hw.dtype == torch.float8_e4m3fn:  # the head is a bf16 layer
+            hw = _dequantise_blocks("lm_head.weight", hw, _get_weight(state, head_keys[0] + "_scale_inv"))
+        hw = hw.to(device=dev, dtype=BF16).contiguous()
         head = Linear(hw.shape[1], hw.shape[0], use_bias=False, weight=hw)
         out = LLM(embed, blocks, norm, head, model.config)
     else:
@@ -214,17 +249,21 @@ def load_hf_weights_into_llm(model: LLM, repo_id: str | dict, revision: str | No
 
 def build_pretrained_llm(repo: str, dtype=None, *, use_cross_attention: bool = False, extra_tokens: int | None = None,
                          tied_extra_embed: bool = False, key=None, use_fp8: bool = True, device=None, tp_rank: int = 0,
-                         tp_size: int = 1) -> LLM:
+                         tp_size: int = 1, fp8_blocks: bool | None = None) -> LLM:
     """xax/arch/llm.py:658-710 for a local checkpoint directory.  ``use_fp8`` (an extension, as in
     LLM.build) makes the projections Fp8Linear layers; the reference reaches the same by swapping
-    them into the module tree."""
+    them into the module tree.  ``fp8_blocks`` makes them Fp8BlockLinear layers; None does so for a block-quantised
+    checkpoint that is not sharded."""
     if extra_tokens is not None or tied_extra_embed:
         raise ValueError("extra tokens are outside the path this library covers")
     if use_cross_attention and key is None:
         raise ValueError("key is required if use_cross_attention is True or extra_tokens is not None.")  # :691-693
-    config = hf_config_to_llm_config(load_hf_config(repo))
+    hf_config = load_hf_config(repo)
+    config = hf_config_to_llm_config(hf_config)
+    if fp8_blocks is None:
+        fp8_blocks = use_fp8 and tp_size == 1 and _block_quantised(hf_config)
     shape = LLM.build(config, key=0 if key is None else key, use_fp8=use_fp8, init_std=0.0, device=device,
-                      tp_rank=tp_rank, tp_size=tp_size)
+                      tp_rank=tp_rank, tp_size=tp_size, fp8_blocks=fp8_blocks)
     llm = load_hf_weights_into_llm(shape, repo, dtype=dtype)
     if use_cross_attention:  # :706-708: the cross-attention weights are freshly initialised
         from .llm import CrossAttentionLLM

@@ -16,7 +16,7 @@ from dataclasses import dataclass, replace
 import torch
 
 from .. import ops
-from ..nn.fp8 import Fp8Linear
+from ..nn.fp8 import Fp8BlockLinear, Fp8Linear
 from .attention import BF16, Embedding, Linear, RMSNorm, SelfAttentionBlock, SwiGLU, TransformerBlock, apply_linear
 
 
@@ -79,10 +79,11 @@ class LLM:
     @classmethod
     def build(cls, config: LLMConfig, *, extra_tokens: int | None = None, tied_extra_embed: bool = False, key=None,
               use_fp8: bool = False, init_std: float | None = None, device=None, tp_rank: int = 0,
-              tp_size: int = 1) -> "LLM":
+              tp_size: int = 1, fp8_blocks: bool = False) -> "LLM":
         """xax/arch/llm.py:96-203.  ``use_fp8`` (an extension: the reference hard-codes False,
         :155) makes q/k/v/out and gate/up/down Fp8Linear layers without bias, which is how the
-        reference reaches an FP8 LLM (by swapping Fp8Linear into the module tree).
+        reference reaches an FP8 LLM (by swapping Fp8Linear into the module tree); ``fp8_blocks``
+        (another extension) makes them Fp8BlockLinear layers, whose 128 x 128 scales are not sharded.
         ``init_std`` draws every weight from N(0, std^2) on the device instead of the
         reference's per-layer uniform init.  ``tp_rank`` / ``tp_size`` build only this rank's
         shard of each weight per get_model_parallel_sharding_spec (same seed on every rank)."""
@@ -97,6 +98,9 @@ class LLM:
         if config.q_heads % tp_size or config.kv_heads % tp_size or width % tp_size:
             raise ValueError(f"tp_size {tp_size} does not divide heads ({config.q_heads}/{config.kv_heads}) or MLP width {width}")
 
+        if fp8_blocks and tp_size > 1:
+            raise ValueError("block-scaled layers are outside the tensor-parallel path of this library")
+
         def shard(w, name):
             dim = tp_shard_dim(name, w.dim())
             if tp_size == 1 or dim is None:
@@ -109,6 +113,8 @@ class LLM:
             if tp_shard_dim(name, 2) == 1 and tp_rank > 0:
                 bias = False  # a row-parallel layer's bias is added once, by rank 0
             b = torch.zeros((w.shape[0],), dtype=BF16, device=dev) if bias else None
+            if fp8_blocks:
+                return Fp8BlockLinear(w.shape[1], w.shape[0], weight=w, bias=b)
             if use_fp8:
                 return Fp8Linear(w.shape[1], w.shape[0], weight=w, bias=b, use_bias=bias)
             return Linear(w.shape[1], w.shape[0], use_bias=bias, weight=w, bias=b)
@@ -223,7 +229,7 @@ class LLM:
 
 def _head_weight(lm_head) -> torch.Tensor:
     w = getattr(lm_head, "weight", None)
-    if not isinstance(w, torch.Tensor) or w.dim() != 2 or isinstance(lm_head, Fp8Linear) or getattr(lm_head, "bias", None) is not None:
+    if not isinstance(w, torch.Tensor) or w.dim() != 2 or isinstance(lm_head, (Fp8Linear, Fp8BlockLinear)) or getattr(lm_head, "bias", None) is not None:
         raise ValueError("the fused loss takes the head as a layer with a bf16 (vocab, hidden) weight and no bias "
                          "(model.lm_head); an arbitrary callable is outside the path this library covers")
     return w.to(BF16)

@@ -9,6 +9,8 @@ Differences from the reference, all deliberate:
     reference's; the output differs from the QDQ formulation by ~4e-3 relative;
   * the weight is quantised once per (weight, scale) and cached instead of on every call
     (xax/nn/fp8.py:336);
+  * ``Fp8BlockLinear`` (not in the reference) scales activations per token and 128 input features and weights per
+    128 x 128 square, the layout of block-quantised checkpoints;
   * ``float8_e5m2`` is served by the free functions (``quantize``, ``dequantize``, ``quantize_dequantize``,
     ``fp8_matmul``: what the reference's tests exercise in both formats); ``Fp8Linear`` itself, i.e. the
     transformer path, takes ``float8_e4m3fn`` only.
@@ -239,6 +241,88 @@ class Fp8Linear:
         if out is not None and hasattr(out, "push_gemm"):
             return out.push_gemm(xq, wq, x_inv, w_inv, self.bias, residual)
         return ops.gemm_fp8(xq, wq, x_inv, w_inv, self.bias, residual, out)
+
+
+class Fp8BlockLinear:
+    """A linear layer in block-scaled e4m3: ``weight`` e4m3 (out_features, in_features) with ``weight_inv`` float32, one
+    multiplier per 128 x 128 square (the last ones cut off at the edge), stands for weight * weight_inv; activations are
+    cast on the way in, one multiplier per token and 128 features.  A token's result therefore depends on no other
+    token, and an outlier costs precision in its own block of 128 alone.
+
+    Built from a bf16 ``weight`` (cast at once, the bf16 tensor is not kept) or from ``weight`` e4m3 and ``weight_inv``
+    as a checkpoint stores them.  in_features must be a multiple of 16, out_features of 8."""
+
+    def __init__(self, in_features: int, out_features: int, *, key=None, use_bias: bool = True,
+                 weight: torch.Tensor | None = None, weight_inv: torch.Tensor | None = None,
+                 bias: torch.Tensor | None = None, device=None):
+        if in_features % 16 or out_features % 8:
+            raise ValueError(f"a block-scaled layer needs in_features ({in_features}) to be a multiple of 16 and "
+                             f"out_features ({out_features}) of 8")
+        self.in_features, self.out_features = in_features, out_features
+        if weight is None:  # the initialisation of Fp8Linear
+            gen = key if isinstance(key, torch.Generator) else torch.Generator(device="cpu").manual_seed(int(key or 0))
+            bound, d = 1.0 / math.sqrt(in_features), _dev(device)
+            weight = ((torch.rand((out_features, in_features), generator=gen) * 2 - 1) * bound).to(torch.bfloat16).to(d)
+            bias = ((torch.rand((out_features,), generator=gen) * 2 - 1) * bound).to(torch.bfloat16).to(d) if use_bias else None
+        if tuple(weight.shape) != (out_features, in_features):
+            raise ValueError(f"weight must be ({out_features}, {in_features}), got {tuple(weight.shape)}")
+        if weight.dtype == torch.float8_e4m3fn:
+            want = (-(-out_features // ops.SCALE_BLOCK), -(-in_features // ops.SCALE_BLOCK))
+            if weight_inv is None or tuple(weight_inv.shape) != want:
+                raise ValueError(f"an e4m3 weight needs weight_inv {want}, one multiplier per 128 x 128 square, got "
+                                 f"{None if weight_inv is None else tuple(weight_inv.shape)}")
+            self.weight, self.weight_inv = weight.contiguous(), weight_inv.to(torch.float32).contiguous()
+        else:
+            if weight_inv is not None:
+                raise ValueError("weight_inv goes with an e4m3 weight")
+            self.weight, self.weight_inv = ops.quantize_blocks(weight.to(torch.bfloat16).contiguous(), ops.SCALE_BLOCK)
+        self.bias = None if bias is None else bias.to(torch.bfloat16).contiguous()
+
+    def __call__(self, x: torch.Tensor, *, residual=None) -> torch.Tensor:
+        """x (..., in_features) -> bf16 (..., out_features); ``residual`` is added in the product's epilogue."""
+        if x.shape[-1] != self.in_features:
+            raise ValueError(f"expected last dimension {self.in_features}, got {x.shape[-1]}")
+        x2 = x.reshape(-1, self.in_features).to(torch.bfloat16)
+        res2 = None if residual is None else residual.reshape(-1, self.out_features)
+        return self.forward_quantized(*ops.quantize_blocks(x2), res2).reshape(*x.shape[:-1], self.out_features)
+
+    def forward_quantized(self, xq: torch.Tensor, x_inv: torch.Tensor, residual=None, out=None) -> torch.Tensor:
+        """The product for activations that quantize_blocks, rmsnorm_blocks or silu_mul_blocks already cast."""
+        return ops.gemm_fp8_blocks(xq, self.weight, x_inv, self.weight_inv, self.bias, residual, out)
+
+
+class StackedBlockLinears:
+    """Several Fp8BlockLinear layers on the same input, their outputs side by side.  Where every layer but the last
+    ends on a whole square the weights are stacked into one operand, so that one product reads the activations once;
+    otherwise each layer writes its own columns."""
+
+    def __init__(self, layers):
+        self.layers = tuple(layers)
+        self._stacked, self._key = None, None
+
+    def _weights(self):
+        key = tuple((t.data_ptr(), t._version) for m in self.layers for t in (m.weight, m.weight_inv, m.bias) if t is not None)
+        if self._key != key:  # a layer's tensor was replaced or written to
+            self._stacked, self._key = None, key
+            if all(m.out_features % ops.SCALE_BLOCK == 0 for m in self.layers[:-1]):
+                q = torch.cat([m.weight.view(torch.uint8) for m in self.layers], 0).view(torch.float8_e4m3fn)
+                bias = None
+                if any(m.bias is not None for m in self.layers):
+                    bias = torch.cat([m.bias if m.bias is not None else m.weight.new_zeros((m.out_features,), dtype=torch.bfloat16)
+                                      for m in self.layers])
+                self._stacked = (q, torch.cat([m.weight_inv for m in self.layers], 0), bias)
+        return self._stacked
+
+    def __call__(self, xq: torch.Tensor, x_inv: torch.Tensor) -> torch.Tensor:
+        stacked = self._weights()
+        if stacked is not None:
+            return ops.gemm_fp8_blocks(xq, stacked[0], x_inv, stacked[1], stacked[2])
+        out = xq.new_empty((xq.shape[0], sum(m.out_features for m in self.layers)), dtype=torch.bfloat16)
+        n0 = 0
+        for m in self.layers:
+            m.forward_quantized(xq, x_inv, out=out[:, n0:n0 + m.out_features])
+            n0 += m.out_features
+        return out
 
 
 def fp8_matmul(a: torch.Tensor, b: torch.Tensor, compute_dtype: torch.dtype = torch.bfloat16,

@@ -34,6 +34,8 @@ class LoRALinear:
         if rank < 1:
             raise ValueError("rank must be at least 1")
         w = linear.weight
+        if w.dtype == torch.float8_e4m3fn:
+            raise ValueError("LoRA goes on a layer that keeps its weight in bf16, not on a block-scaled one")
         gen = key if isinstance(key, torch.Generator) else torch.Generator(device="cpu").manual_seed(int(key or 0))
         a = (torch.randn((w.shape[1], rank), generator=gen) / math.sqrt(float(w.shape[1]))).to(w.dtype).to(w.device)
         b = torch.zeros((rank, w.shape[0]), dtype=w.dtype, device=w.device)
