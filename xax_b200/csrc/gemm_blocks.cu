@@ -63,6 +63,18 @@ __device__ __forceinline__ void warpgroup_sync(int which) {
     asm volatile("bar.sync 2, 128;" ::: "memory");
 }
 
+// Shared-memory loads that stay where they are written.
+__device__ __forceinline__ float lds_f1(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
 // bf16(f + bias + residual) of eight neighbouring columns, 16 bytes.
 __device__ __forceinline__ void finish8(const GemmBlocksParams& p, float (&f)[8], int m, int n) {
   if (p.bias) {
@@ -109,25 +121,26 @@ __device__ __forceinline__ void fma2(float& a, float& b, uint32_t x, uint32_t y,
 // product over).
 // What bounds it is the operand bytes that an SM keeps in flight, so the ring takes all the shared memory that the CTAs
 // which will be resident together leave (`stages`, from the launcher).
-template <int NT>
+// kAlone: for launches of at most one CTA an SM, which leaves NT = 128 room for 32-column readouts and four buffers.
+template <int NT, bool kAlone>
 struct BlocksDecodeCfg {
   static constexpr bool kTokenRows = NT == 128;            // the token is the accumulator's row, else the weight row is
   static constexpr int kGroups = NT == 128 ? 2 : 1;        // promoting warpgroups
   static constexpr int kCols = NT / kGroups;               // accumulator columns per promoting thread
   static constexpr int kThreads = NT == 128 ? 384 : 224;
-  // Registers of NT = 128: two CTAs of 384 threads start with 80 a thread; the warpgroup of the producer and the
-  // issuer gives up what the promoting ones need.
-  static constexpr bool kMoveRegs = NT == 128;
+  // Registers of two CTAs of NT = 128: their 384 threads start with 80 each; the warpgroup of the producer and the
+  // issuers gives up what the promoting ones need.
+  static constexpr bool kMoveRegs = NT == 128 && !kAlone;
   static constexpr int kPromoteRegs = 104, kIssueRegs = 32;
   static_assert(kGroups * kPromoteRegs + kIssueRegs <= 3 * 80, "register split");
-  static constexpr int kCtasPerSm = NT == 16 ? 3 : 2;      // at most: registers, tensor memory
+  static constexpr int kCtasPerSm = kAlone ? 1 : NT == 16 ? 3 : 2;  // at most: registers, tensor memory
   static constexpr int kWeightBytes = kBM * kBKBytes;
   static constexpr int kStageBytes = kWeightBytes + NT * kBKBytes;
   static constexpr int kMaxStages = 12;
-  static constexpr int kBufs = NT == 32 ? 3 : NT == 128 ? 2 : 4;  // tensor-memory buffers of NT columns
+  static constexpr int kBufs = NT == 32 ? 3 : kMoveRegs ? 2 : 4;  // tensor-memory buffers of NT columns
   static constexpr int kTmemCols = NT == 32 ? 128 : kBufs * NT;
   static constexpr int kScaleBlocks = 16;                  // K blocks whose multipliers are staged at a time
-  static constexpr int kLoad = NT == 16 || NT == 128 ? 16 : 32;  // columns per readout (what the registers allow)
+  static constexpr int kLoad = NT == 16 || kMoveRegs ? 16 : 32;  // columns per readout (what the registers allow)
   static constexpr int kPartFloats = kBM + 4;              // floats per token of a CTA's part of the result
   static constexpr int kExtraBytes = kScaleBlocks * NT * 4 + (2 * kMaxStages + 1) * 8;
   static constexpr int kSmemPerSm = 228 * 1024, kSmemReserved = 1024;
@@ -146,11 +159,11 @@ struct BlocksDecodeCfg {
   static_assert(kCtasPerSm * kTmemCols <= 512, "tensor memory");
 };
 
-template <int NT>
-__global__ void __launch_bounds__(BlocksDecodeCfg<NT>::kThreads, BlocksDecodeCfg<NT>::kCtasPerSm)
+template <int NT, bool kAlone>
+__global__ void __launch_bounds__(BlocksDecodeCfg<NT, kAlone>::kThreads, BlocksDecodeCfg<NT, kAlone>::kCtasPerSm)
 gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                           const GemmBlocksParams p, const int S, const int stages) {
-  using Cfg = BlocksDecodeCfg<NT>;
+  using Cfg = BlocksDecodeCfg<NT, kAlone>;
   constexpr int kBufs = Cfg::kBufs, kPromoteWarps = 4 * Cfg::kGroups;
   constexpr uint32_t kIdesc = umma_idesc(kFmtE4M3, kFmtE4M3, 0, 0, kBM, NT);
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -186,6 +199,10 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
   pdl_trigger();  // tensor memory is allocated: the next kernel may be scheduled
+  // The first weight tiles are asked into L2 while the previous kernel ends (nothing in flight writes weights, and L2 is
+  // the point of coherence); everything that reads or writes global memory for good waits for it.
+  if (warp == kPromoteWarps && lane == 0)
+    for (int i = 0; i < min(4, nkb); ++i) tma_prefetch_l2_2d(&tmap_w, (kb0 + i) * kBKBytes, n0);
   pdl_wait();
 
   if (warp >= kPromoteWarps) {
@@ -263,8 +280,7 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
       ok = __all_sync(0xffffffffu, ok);  // (a warp that gave up still takes part in the barriers above)
       if (ok) {
         tc_fence_after_sync();
-        const float* sc = scales + in_chunk * NT + (Cfg::kTokenRows ? quarter * 32 + lane : 0);
-        const float row_scale = Cfg::kTokenRows ? *sc : 0.0f;
+        const uint32_t sc = smem_u32(scales + in_chunk * NT + (Cfg::kTokenRows ? quarter * 32 + lane : 0));
         const uint32_t from = taddr + buf * NT;
 #pragma unroll
         for (int c = 0; c < Cfg::kCols; c += Cfg::kLoad) {
@@ -273,6 +289,16 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
             tmem_ld_x32(from + c, r);
           else
             tmem_ld_x16(from + c, r);
+          // the columns' multipliers, on their way together with the products (left to the compiler each is read right
+          // before its use: 770 cycles a block for 64 tokens)
+          float4 mul[Cfg::kTokenRows ? 1 : Cfg::kLoad / 4];
+          if constexpr (Cfg::kTokenRows) {
+            const float v = lds_f1(sc);
+            mul[0] = make_float4(v, v, v, v);
+          } else {
+#pragma unroll
+            for (int j = 0; j < Cfg::kLoad / 4; ++j) mul[j] = lds_f4(sc + (c + 4 * j) * 4);
+          }
           tmem_ld_wait();
           if (c + Cfg::kLoad == Cfg::kCols) {
             tc_fence_before_sync();
@@ -281,10 +307,9 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
           }
 #pragma unroll
           for (int j = 0; j < Cfg::kLoad; j += 4) {
-            const float4 s4 = Cfg::kTokenRows ? make_float4(row_scale, row_scale, row_scale, row_scale)
-                                              : *reinterpret_cast<const float4*>(sc + c + j);
-            fma2(acc[c + j], acc[c + j + 1], r[j], r[j + 1], s4.x, s4.y);
-            fma2(acc[c + j + 2], acc[c + j + 3], r[j + 2], r[j + 3], s4.z, s4.w);
+            const float4 m4 = mul[Cfg::kTokenRows ? 0 : j / 4];
+            fma2(acc[c + j], acc[c + j + 1], r[j], r[j + 1], m4.x, m4.y);
+            fma2(acc[c + j + 2], acc[c + j + 3], r[j + 2], r[j + 3], m4.z, m4.w);
           }
         }
       }
@@ -369,27 +394,34 @@ static int pick_split(long long tiles, int num_k_blocks, int num_sms) {
   return s;
 }
 
-template <int NT>
-static int launch_decode(const Ctx* ctx, cudaStream_t stream, const GemmBlocksParams& p) {
-  using Cfg = BlocksDecodeCfg<NT>;
+template <int NT, bool kAlone>
+static int launch_decode_as(const Ctx* ctx, cudaStream_t stream, const GemmBlocksParams& p, int tiles_n, int tiles_m, int S,
+                            int per_sm) {
+  using Cfg = BlocksDecodeCfg<NT, kAlone>;
   CUtensorMap tw, tx;
   if (int rc = make_tmap_2d(ctx, &tw, p.b, 1, (uint64_t)p.K, (uint64_t)p.N, (uint64_t)p.ldb, kBKBytes, kBM)) return rc;
   if (int rc = make_tmap_2d(ctx, &tx, p.a, 1, (uint64_t)p.K, (uint64_t)p.M, (uint64_t)p.lda, kBKBytes, NT)) return rc;
-  if (int rc = ensure_dynamic_smem<gemm_blocks_decode_kernel<NT>>(ctx, Cfg::smem_bytes(Cfg::stages_for(1)),
-                                                                  "gemm_blocks_decode_kernel"))
+  if (int rc = ensure_dynamic_smem<gemm_blocks_decode_kernel<NT, kAlone>>(ctx, Cfg::smem_bytes(Cfg::stages_for(1)),
+                                                                          "gemm_blocks_decode_kernel"))
     return rc;
-  const int tiles_n = (p.N + kBM - 1) / kBM, tiles_m = (p.M + NT - 1) / NT;
-  const int S = pick_split((long long)tiles_n * tiles_m, p.num_k_blocks, ctx->num_sms);
-  const long long ctas = (long long)tiles_n * tiles_m * S;
-  const int per_sm = (int)min((long long)Cfg::kCtasPerSm, (ctas + ctx->num_sms - 1) / ctx->num_sms);
-  const int stages = Cfg::stages_for(per_sm);
-  cudaError_t e = launch_kernel(gemm_blocks_decode_kernel<NT>, dim3((unsigned)(tiles_n * S), (unsigned)tiles_m),
+  const int stages = Cfg::stages_for(per_sm < Cfg::kCtasPerSm ? per_sm : Cfg::kCtasPerSm);
+  cudaError_t e = launch_kernel(gemm_blocks_decode_kernel<NT, kAlone>, dim3((unsigned)(tiles_n * S), (unsigned)tiles_m),
                                 dim3(Cfg::kThreads), Cfg::smem_bytes(stages), stream, (unsigned)S, tw, tx, p, S, stages);
   if (e != cudaSuccess) {
     set_last_error("gemm_blocks_decode_kernel launch: %s", cudaGetErrorString(e));
     return XAXB_LAUNCH_FAILED;
   }
   return check_launch("gemm_blocks_decode_kernel");
+}
+
+template <int NT>
+static int launch_decode(const Ctx* ctx, cudaStream_t stream, const GemmBlocksParams& p) {
+  const int tiles_n = (p.N + kBM - 1) / kBM, tiles_m = (p.M + NT - 1) / NT;
+  const int S = pick_split((long long)tiles_n * tiles_m, p.num_k_blocks, ctx->num_sms);
+  const long long ctas = (long long)tiles_n * tiles_m * S;
+  const int per_sm = (int)((ctas + ctx->num_sms - 1) / ctx->num_sms < 4 ? (ctas + ctx->num_sms - 1) / ctx->num_sms : 4);
+  if (NT == 128 && per_sm == 1) return launch_decode_as<NT, NT == 128>(ctx, stream, p, tiles_n, tiles_m, S, per_sm);
+  return launch_decode_as<NT, false>(ctx, stream, p, tiles_n, tiles_m, S, per_sm);
 }
 
 // ---------------------------------------------------------------------------------------
