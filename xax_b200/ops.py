@@ -256,7 +256,8 @@ def _check_rows(what: str, t: torch.Tensor, dtype, name: str, shape=None) -> Non
 
 def _device_of(t: torch.Tensor) -> int:
     """The current device if ``t`` is on it, else -2 (on which no tensor is, so that the helpers get to refuse it)."""
-    return t.get_device() if t.is_cuda and t.get_device() == torch.cuda.current_device() else -2
+    device = t.get_device()  # -1 for a CPU tensor
+    return device if device >= 0 and device == torch.cuda.current_device() else -2
 
 
 def quantize_blocks(x: torch.Tensor, block_rows: int = 1):
@@ -271,7 +272,7 @@ def quantize_blocks(x: torch.Tensor, block_rows: int = 1):
         raise ValueError(f"quantize_blocks: block_rows must be 1 or {SCALE_BLOCK}, got {block_rows}")
     rows, cols = x.shape
     q = torch.empty_like(x, dtype=E4M3)
-    inv = x.new_empty((-(-rows // block_rows), -(-cols // SCALE_BLOCK)), dtype=F32)
+    inv = x.new_empty(-(-rows // block_rows), -(-cols // SCALE_BLOCK), dtype=F32)
     if rows == 0:
         return q, inv
     ctx, st, lib = _lib.call_state(dev)
@@ -312,7 +313,7 @@ def gemm_fp8_blocks(a_q, b_q, a_inv, b_inv, bias=None, residual=None, out=None):
             _check_rows(what, residual, BF16, "residual", (M, N))
         res_ptr, ldr = residual.data_ptr(), residual.stride(0) if M > 1 else N
     if out is None:
-        out = a_q.new_empty((M, N), dtype=BF16)
+        out = a_q.new_empty(M, N, dtype=BF16)
     else:
         _check_rows(what, out, BF16, "out", (M, N))
     if M == 0:
@@ -344,7 +345,7 @@ def rmsnorm_blocks(x, weight, eps, *, residual=None):
         total = torch.empty_like(x)
         res_ptr, total_ptr = residual.data_ptr(), total.data_ptr()
     q = torch.empty_like(x, dtype=E4M3)
-    inv = x.new_empty((rows, -(-cols // SCALE_BLOCK)), dtype=F32)
+    inv = x.new_empty(rows, -(-cols // SCALE_BLOCK), dtype=F32)
     if rows == 0:
         return total, q, inv
     ctx, st, lib = _lib.call_state(dev)
@@ -363,8 +364,8 @@ def silu_mul_blocks(gate_up, dim: int):
     rows, ld = gate_up.shape
     if dim <= 0 or ld != 2 * dim:
         raise ValueError(f"silu_mul_blocks: gate_up must be [rows, 2 * {dim}], got {tuple(gate_up.shape)}")
-    q = gate_up.new_empty((rows, dim), dtype=E4M3)
-    inv = gate_up.new_empty((rows, -(-dim // SCALE_BLOCK)), dtype=F32)
+    q = gate_up.new_empty(rows, dim, dtype=E4M3)
+    inv = gate_up.new_empty(rows, -(-dim // SCALE_BLOCK), dtype=F32)
     if rows == 0:
         return q, inv
     ctx, st, lib = _lib.call_state(dev)
