@@ -375,6 +375,34 @@ def test_two_streams_at_once():
         assert all(torch.equal(g, want[i]) for g in got[i])
 
 
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 values: the last rows come out as they do alone."""
+    from xax_b200 import ops
+
+    def tail_matches(whole, part):
+        for w, p in zip(whole, part):
+            assert torch.equal(w[-p.shape[0]:].view(torch.uint8), p.view(torch.uint8))
+
+    rows, cols, last = 131100, 16416, 5  # 2.15e9 values; a width that is no multiple of 128
+    x = torch.empty((rows, cols), dtype=BF16, device="cuda")
+    x[:-last] = 1.0
+    x[-last:] = activations(last, cols, 1)
+    end = x[-last:].clone()
+    tail_matches(ops.quantize_blocks(x), ops.quantize_blocks(end))
+    w = torch.ones((cols,), dtype=BF16, device="cuda")
+    tail_matches(ops.rmsnorm_blocks(x, w, 1e-6, residual=x), ops.rmsnorm_blocks(end, w, 1e-6, residual=end))
+    tail_matches(ops.silu_mul_blocks(x, cols // 2), ops.silu_mul_blocks(end, cols // 2))
+    del x
+    M, N, K = 262300, 8200, 144  # 2.15e9 results
+    a_q, a_inv, b_q, b_inv = operands(300, N, K, 1)
+    big_q, big_inv = a_q.view(torch.uint8)[:1].expand(M, K).contiguous().view(E4M3), a_inv[:1].expand(M, 2).contiguous()
+    big_q.view(torch.uint8)[-300:], big_inv[-300:] = a_q.view(torch.uint8), a_inv
+    residual = torch.ones((M, N), dtype=BF16, device="cuda")
+    out = ops.gemm_fp8_blocks(big_q, b_q, big_inv, b_inv, None, residual)
+    check_product(out[-300:], a_q, a_inv, b_q, b_inv, None, residual[-300:])
+    check_product(out[:2], big_q[:2], big_inv[:2], b_q, b_inv, None, residual[:2])
+
+
 # ---------------------------------------------------------------------------------------
 # refusals and small calls
 
