@@ -34,7 +34,7 @@ __device__ __forceinline__ void promote_sync() {
 }
 
 // mbar_wait for barriers that complete within a microsecond: polls before it turns to the clock and the limit, which
-// lives in global memory (reading it once cost a K block of the pair kernel a thousand cycles).
+// lives in global memory.
 __device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* d_status,
                                                int code) {
 #pragma unroll 1
@@ -108,7 +108,8 @@ __device__ __forceinline__ void fma2(float& a, float& b, uint32_t x, uint32_t y,
 // columns, so a decode step moves 16 KB of weights and only NT * 128 bytes of activations per K block.  A cluster of S
 // CTAs shares the K blocks of one tile; each CTA pushes its part of the result into the shared memory of the CTA that
 // owns the token, which adds the parts in rank order (no atomics: the same bits every time).  (Pulling the parts took
-// S remote round trips per item: 7000 of 38000 cycles for 128 x 4096 x 14336, S = 4.)
+// S remote round trips per item, 7000 of 38000 cycles for 128 x 4096 x 14336, S = 4; one bulk copy per owner in place of
+// the threads' 16-byte pushes 20.0 us against 19.0.)
 //   promoting warps  thread = weight row; acc[t] += partial[t] * (a_inv[t, kb] * b_inv[kb]) in float32 registers.  With
 //                    NT = 128 the operands change places: thread = token, two warpgroups of 64 weight rows each, and the
 //                    combined multiplier is one value a thread instead of one a column.
@@ -120,7 +121,10 @@ __device__ __forceinline__ void fma2(float& a, float& b, uint32_t x, uint32_t y,
 // arriving on the stage that the block will use) and one closes it (the commit on done[s] frees the stage and hands the
 // product over).
 // What bounds it is the operand bytes that an SM keeps in flight, so the ring takes all the shared memory that the CTAs
-// which will be resident together leave (`stages`, from the launcher).
+// which will be resident together leave (`stages`, from the launcher).  Measured (graph of launches, operands past L2):
+// 1 x 28672 x 4096 20.9 us = 5.6 TB/s, 0.86 of the copy rate (224 tiles on 148 SMs; the rest is that imbalance);
+// 64 x 4096 x 14336 16.4, 128 x 4096 x 14336 19.0, 64 x 2048 x 5632 8.2, 1 x 4096 x 4096 5.3 us, of which start, first
+// copies, the two cluster barriers and the pushes are 3 (16 tokens) to 6 us (128).
 // kAlone: for launches of at most one CTA an SM, which leaves NT = 128 room for 32-column readouts and four buffers.
 template <int NT, bool kAlone>
 struct BlocksDecodeCfg {
@@ -431,13 +435,20 @@ static int launch_decode(const Ctx* ctx, cudaStream_t stream, const GemmBlocksPa
 // 128 columns each: one weight square) read it out, scale it and add it to float32 registers while the tensor
 // core fills the other buffer.
 //
-// Per 128-byte K block the tensor core needs 512 cycles, reading the buffer out 256, the packed multiply-adds 128 issue
-// slots: the promotion hides behind the MMAs as long as neither side waits for the other's bookkeeping.  Issuing is what
-// takes time there (a barrier test, an MMA or a commit costs its thread about a hundred cycles), so
+// Per 128-byte K block the tensor core needs 512 cycles and the packed multiply-adds of two warps per scheduler 256, so the
+// promotion could hide behind the MMAs; what bounds the kernel is the turnaround of a buffer: 350 cycles from its
+// release until the issuing thread sees it, 512 of MMAs, 400 from the commit until the promoting warps see that, 330 until
+// they have read it, shared by two buffers: about 900 a block, 62 % of the tensor pipe (without readout and promotion
+// 341 us of 433, and no less with a quarter of the MMAs).  4096 x 28672 x 4096: 421 us = 2.28 PFLOP/s in a graph, 480
+// under the power cap; 2048 x 8192 x 2048: 37.2.  Not faster: 128 x 256 tiles on single CTAs, whose releases are local but
+// which read half as much again out of L2 (467 against 419 us); halves of 128 columns with barriers of their own (578);
+// opening the next block before the last columns of this one are added (490).  To keep the turnaround short
 //   * two warps issue, one the even and one the odd K blocks (different buffers, nothing to order between them);
 //   * one barrier opens a K block: full[s] counts both CTAs' copies AND the 16 warps that free the buffer, the latter
 //     arriving on the stage that the block two further on will use;
-//   * one commit closes it, multicast to both CTAs: done[s] frees the stage and hands the product over.
+//   * one commit closes it, multicast to both CTAs: done[s] frees the stage and hands the product over;
+//   * a spare warp brings the multipliers through shared memory (loads by the promoting threads, however early, had them
+//     wait for L2 behind every barrier: 594 us).
 // Registers: three warpgroups start with 168 each; the issuing one gives up what the promoting ones need.
 constexpr int kPairThreads = 384;
 constexpr int kPairLaunchRegs = 168, kPairPromoteRegs = 192, kPairIssueRegs = 120;
