@@ -457,3 +457,15 @@ def test_arguments_are_checked():
     for call in bad:
         with pytest.raises(ValueError):
             call()
+
+
+def test_silu_mul_blocks_where_the_sigmoid_is_denormal():
+    """Gates from -87.3 down have a sigmoid below the smallest normal float32; their product with a large up counts."""
+    from xax_b200 import ops
+
+    gu = torch.empty((4, 512), dtype=BF16, device="cuda")
+    gu[:, :256] = torch.linspace(-88.5, -84.0, 256, device="cuda")  # (e^88.5 is the last that float32 holds)
+    gu[:, 256:] = torch.tensor([1.0, 1e10, 1e30, 3e38], device="cuda")[:, None]
+    q, inv = ops.silu_mul_blocks(gu, 256)
+    g, u = gu[:, :256].to(F64), gu[:, 256:].to(F64)
+    check_cast(g * torch.sigmoid(g) * u, q, inv, 1, D_SILU)

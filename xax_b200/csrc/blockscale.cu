@@ -209,20 +209,21 @@ __global__ void __launch_bounds__(NT) rmsnorm_blocks_kernel(const __nv_bfloat16*
 
 // ---- silu(gate) * up, gate and up the two halves of a row of the fused gate | up product.
 
-// 1 / (1 + e^x) to a few units: e^x = 2^h (1 + l) with h = x log2 e rounded and l = x - h ln 2, from the approximate
-// exponential and reciprocal (2^-22 each).  x is kept from -88 up, where e^x is nothing beside 1, and h up to 127, past
-// which the result is below the smallest normal float; NaN comes back in the product with the gate.
-__device__ __forceinline__ float one_over_one_plus_exp(float x) {
+// 4 / (1 + e^x) to a few units: e^x = 2^h (1 + l) with h = x log2 e rounded and l = x - h ln 2, from the approximate
+// exponential and reciprocal (2^-22 each).  x is kept from -88 up, where e^x is nothing beside 1, and h below 128; past
+// that e^x is infinite in float32 and the result 0.  NaN comes back in the product with the gate.  (Four times the value,
+// since the reciprocal itself would be denormal, and flushed, from x = 87.3 up, where gate times it is not yet.)
+__device__ __forceinline__ float four_over_one_plus_exp(float x) {
   x = fmaxf(x, -88.0f);
-  const float h = fminf(x * 1.4426950408889634f, 127.0f);
+  const float h = fminf(x * 1.4426950408889634f, 127.99999f);
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(h));
   e = fmaf(e, fmaf(h, -0.6931471805599453f, x), e);
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(e, 0.25f, 0.25f)));
   return r;
 }
 
-__device__ __forceinline__ float silu_mul(float g, float u) { return g * one_over_one_plus_exp(-g) * u; }
+__device__ __forceinline__ float silu_mul(float g, float u) { return 0.25f * g * four_over_one_plus_exp(-g) * u; }
 
 // A grid of resident CTAs walks the pieces; the next piece's loads are under way while one is computed.  An exponential, a
 // reciprocal and a dozen more instructions per value take about as long as its bytes (4099 x 5632: 20.6 us = 5.6 TB/s, 0.85
