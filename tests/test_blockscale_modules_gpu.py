@@ -218,3 +218,54 @@ def test_block_quantised_checkpoint(tmp_path):
     checkpoint(m, tmp_path, size=(64, 128))
     with pytest.raises(ValueError, match="weight_block_size"):
         build_pretrained_llm(str(tmp_path))
+
+
+def test_stacked_weights_are_the_layers_own():
+    """Layers that the library builds share one operand: no second copy, no stale one, and layers of the user's stay theirs."""
+    from xax_b200 import Fp8BlockLinear, SwiGLU, ops
+
+    x = randn(9, 256, seed=1)
+    xq, x_inv = ops.quantize_blocks(x)
+
+    def each(mlp):
+        return torch.cat([m.forward_quantized(xq, x_inv) for m in (mlp.gate, mlp.up)], 1)
+
+    mlp = SwiGLU.build(256, 384, key=3, use_bias=True, fp8_blocks=True)
+    assert mlp.gate.weight.untyped_storage().data_ptr() == mlp.up.weight.untyped_storage().data_ptr()
+    assert mlp._gate_up_stack()._weights()[0].data_ptr() == mlp.gate.weight.data_ptr()
+    assert same(mlp._gate_up_stack()(xq, x_inv), each(mlp))
+    other, other_inv = ops.quantize_blocks(randn(384, 256, seed=5, std=0.05), 128)
+    for write in (lambda: mlp.up.weight.data.copy_(other), lambda: mlp.up.weight_inv.data.copy_(other_inv),
+                  lambda: setattr(mlp.gate, "weight", other), lambda: mlp.gate.bias.data.zero_(),
+                  lambda: setattr(mlp.up, "bias", None)):
+        before = mlp._gate_up_stack()(xq, x_inv)
+        write()
+        after = mlp._gate_up_stack()(xq, x_inv)
+        assert same(after, each(mlp)) and not same(after, before)
+
+    gate, up = (Fp8BlockLinear(256, 384, key=k, use_bias=False) for k in (1, 2))
+    held = gate.weight
+    with torch.inference_mode():
+        mine = SwiGLU(gate, up, Fp8BlockLinear(384, 256, key=4, use_bias=False))
+        first = mine.forward_tokens(x, 1, 9)
+    held.copy_(other)
+    assert gate.weight is held and not same(mine.forward_tokens(x, 1, 9), first)
+    assert same(mine._gate_up_stack()(xq, x_inv), each(mine))
+
+
+def test_first_call_captured():
+    """A module whose first call is captured answers alike before, in and after the replay."""
+    from xax_b200 import Fp8BlockLinear, SwiGLU
+
+    x = randn(9, 256, seed=1)
+    warm, mlp = (SwiGLU.build(256, 384, key=3, fp8_blocks=True) for _ in range(2))
+    want = warm.forward_tokens(x, 1, 9)
+    own = SwiGLU(*(Fp8BlockLinear(i, o, key=k, use_bias=False) for i, o, k in ((256, 384, 4), (256, 384, 5), (384, 256, 6))))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, got_own = mlp.forward_tokens(x, 1, 9), own.forward_tokens(x, 1, 9)
+    eager, eager_own = mlp.forward_tokens(x, 1, 9), own.forward_tokens(x, 1, 9)
+    graph.replay()
+    assert same(eager, want) and same(got, want)
+    assert same(got_own, eager_own)

@@ -25,7 +25,7 @@ from typing import Literal, NotRequired, TypedDict
 import torch
 
 from .. import ops
-from ..nn.fp8 import Fp8BlockLinear, Fp8Linear, Fp8Scales, StackedBlockLinears, init_fp8_scales
+from ..nn.fp8 import Fp8BlockLinear, Fp8Linear, Fp8Scales, StackedBlockLinears, init_fp8_scales, stack_block_weights
 from ..nn.lora import LoRALinear
 
 BF16 = torch.bfloat16
@@ -167,7 +167,12 @@ class SwiGLU:
         else:
             mk = lambda i, o, k: Linear(i, o, use_bias=use_bias, key=k, device=device)  # noqa: E731
         return cls(mk(embed_dim, hidden_dim, seed + 1), mk(embed_dim, hidden_dim, seed + 2),
-                   mk(hidden_dim, embed_dim, seed + 3))
+                   mk(hidden_dim, embed_dim, seed + 3)).stack_weights()
+
+    def stack_weights(self) -> "SwiGLU":
+        """Block-scaled gate and up layers that this library has just made share one operand."""
+        stack_block_weights((self.gate, self.up))
+        return self
 
     def is_fp8(self) -> bool:
         return all(isinstance(m, Fp8Linear) and m.use_fp8 for m in (self.gate, self.up, self.down))
@@ -404,7 +409,12 @@ class SelfAttentionBlock:
         return cls(mk(embed_dim, qd, seed + 1), mk(embed_dim, kd, seed + 2), mk(embed_dim, kd, seed + 3),
                    mk(qd, embed_dim, seed + 4), rope, qn, kn, sinks, num_heads=num_heads, num_kv_heads=kv, head_dim=hd,
                    causal=causal, local_window_size=None if context_length is None else context_length - 1,  # :660
-                   use_fp8=use_fp8)
+                   use_fp8=use_fp8).stack_weights()
+
+    def stack_weights(self) -> "SelfAttentionBlock":
+        """Block-scaled q, k and v layers that this library has just made share one operand."""
+        stack_block_weights((self.q_proj, self.k_proj, self.v_proj))
+        return self
 
     @property
     def embed_dim(self) -> int:

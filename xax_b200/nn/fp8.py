@@ -291,26 +291,56 @@ class Fp8BlockLinear:
         return ops.gemm_fp8_blocks(xq, self.weight, x_inv, self.weight_inv, self.bias, residual, out)
 
 
+def stack_block_weights(layers) -> None:
+    """Moves the weights of new Fp8BlockLinear layers on the same input into one operand, of which each layer keeps its
+    slice, so that StackedBlockLinears runs one product and no weight is kept twice.  Does nothing where a layer but the
+    last ends inside a square, or where only some have a bias.  For layers whose tensors nobody else holds yet."""
+    if not all(isinstance(m, Fp8BlockLinear) for m in layers) or any(m.out_features % ops.SCALE_BLOCK for m in layers[:-1]):
+        return
+    if len({m.bias is None for m in layers}) > 1:
+        return
+    q = torch.cat([m.weight.view(torch.uint8) for m in layers]).view(torch.float8_e4m3fn)
+    inv = torch.cat([m.weight_inv for m in layers])
+    bias = None if layers[0].bias is None else torch.cat([m.bias for m in layers])
+    n0 = s0 = 0
+    for m in layers:
+        n1, s1 = n0 + m.out_features, s0 + m.weight_inv.shape[0]
+        m.weight, m.weight_inv = q[n0:n1], inv[s0:s1]
+        if bias is not None:
+            m.bias = bias[n0:n1]
+        n0, s0 = n1, s1
+
+
+def _joined(tensors):
+    """The tensors as one, if each begins where the one before ends in the same memory; else None."""
+    first, at = tensors[0], tensors[0].data_ptr()
+    for t in tensors:
+        if t.data_ptr() != at or not t.is_contiguous() or t.untyped_storage().data_ptr() != first.untyped_storage().data_ptr():
+            return None
+        at += t.numel() * t.element_size()
+    return first.as_strided((sum(t.shape[0] for t in tensors), *first.shape[1:]), first.stride())
+
+
 class StackedBlockLinears:
-    """Several Fp8BlockLinear layers on the same input, their outputs side by side.  Where every layer but the last
-    ends on a whole square the weights are stacked into one operand, so that one product reads the activations once;
-    otherwise each layer writes its own columns."""
+    """Several Fp8BlockLinear layers on the same input, their outputs side by side.  Layers whose weights lie one behind the
+    other (stack_block_weights) are one operand of one product, which reads the activations once; of others each writes its
+    own columns.  Nothing is copied: a weight that is written to or replaced counts from the next call on."""
 
     def __init__(self, layers):
         self.layers = tuple(layers)
         self._stacked, self._key = None, None
 
     def _weights(self):
-        key = tuple((t.data_ptr(), t._version) for m in self.layers for t in (m.weight, m.weight_inv, m.bias) if t is not None)
-        if self._key != key:  # a layer's tensor was replaced or written to
-            self._stacked, self._key = None, key
-            if all(m.out_features % ops.SCALE_BLOCK == 0 for m in self.layers[:-1]):
-                q = torch.cat([m.weight.view(torch.uint8) for m in self.layers], 0).view(torch.float8_e4m3fn)
-                bias = None
-                if any(m.bias is not None for m in self.layers):
-                    bias = torch.cat([m.bias if m.bias is not None else m.weight.new_zeros((m.out_features,), dtype=torch.bfloat16)
-                                      for m in self.layers])
-                self._stacked = (q, torch.cat([m.weight_inv for m in self.layers], 0), bias)
+        # The views hold the memory, so as long as they live these addresses mean the same memory.
+        key = [t.data_ptr() for m in self.layers for t in (m.weight, m.weight_inv, m.bias) if t is not None]
+        if self._key != key:
+            biases = [m.bias for m in self.layers if m.bias is not None]
+            q, inv, bias = None, None, None
+            if all(m.out_features % ops.SCALE_BLOCK == 0 for m in self.layers[:-1]) and len(biases) in (0, len(self.layers)):
+                q, inv = _joined([m.weight for m in self.layers]), _joined([m.weight_inv for m in self.layers])
+                bias = _joined(biases) if biases else None
+            self._stacked = None if q is None or inv is None or (biases and bias is None) else (q, inv, bias)
+            self._key = key if self._stacked is not None else None
         return self._stacked
 
     def __call__(self, xq: torch.Tensor, x_inv: torch.Tensor) -> torch.Tensor:
