@@ -226,7 +226,7 @@ __device__ __forceinline__ float four_over_one_plus_exp(float x) {
 __device__ __forceinline__ float silu_mul(float g, float u) { return 0.25f * g * four_over_one_plus_exp(-g) * u; }
 
 // A grid of resident CTAs walks the pieces; the next piece's loads are under way while one is computed.  An exponential, a
-// reciprocal and a dozen more instructions per value take about as long as its bytes (4099 x 5632: 20.6 us = 5.6 TB/s, 0.85
+// reciprocal and a dozen more instructions per value take about as long as its bytes (4099 x 5632: 20.5 us = 5.7 TB/s, 0.86
 // of the copy rate, with 55 % of the special-function unit and 70 % of the issue slots; 27.5 us with the library's
 // exponential and division or with approximations that treat denormals).
 __global__ void __launch_bounds__(256) silu_mul_blocks_kernel(const __nv_bfloat16* __restrict__ gate_up, int64_t ld,
