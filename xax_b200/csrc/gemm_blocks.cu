@@ -123,7 +123,7 @@ __device__ __forceinline__ void fma2(float& a, float& b, uint32_t x, uint32_t y,
 // What bounds it is the operand bytes that an SM keeps in flight, so the ring takes all the shared memory that the CTAs
 // which will be resident together leave (`stages`, from the launcher).  Measured (graph of launches, operands past L2):
 // 1 x 28672 x 4096 20.9 us = 5.6 TB/s, 0.86 of the copy rate (224 tiles on 148 SMs; the rest is that imbalance);
-// 64 x 4096 x 14336 16.4, 128 x 4096 x 14336 19.0, 64 x 2048 x 5632 8.2, 1 x 4096 x 4096 5.3 us, of which start, first
+// 64 x 4096 x 14336 15.9, 128 x 4096 x 14336 18.9, 64 x 2048 x 5632 7.9, 1 x 4096 x 4096 5.3 us, of which start, first
 // copies, the two cluster barriers and the pushes are 3 (16 tokens) to 6 us (128).
 // kAlone: for launches of at most one CTA an SM, which leaves NT = 128 room for 32-column readouts and four buffers.
 template <int NT, bool kAlone>
@@ -146,20 +146,30 @@ struct BlocksDecodeCfg {
   static constexpr int kScaleBlocks = 16;                  // K blocks whose multipliers are staged at a time
   static constexpr int kLoad = NT == 16 || kMoveRegs ? 16 : 32;  // columns per readout (what the registers allow)
   static constexpr int kPartFloats = kBM + 4;              // floats per token of a CTA's part of the result
-  static constexpr int kExtraBytes = kScaleBlocks * NT * 4 + (2 * kMaxStages + 1) * 8;
+  static constexpr int kPartBytes = (kTokenRows ? 1 : 2) * NT * kPartFloats * 4;  // (two: one to turn it round in)
+  static constexpr int kExtraBytes = kScaleBlocks * NT * 4 + (2 * kMaxStages + 2) * 8;
   static constexpr int kSmemPerSm = 228 * 1024, kSmemReserved = 1024;
+  // The CTAs of a cluster (one on an SM) keep the parts beside the ring, so that none waits for another's ring before it
+  // pushes (64 x 4096 x 14336: 16.5 -> 16.0 us, 64 x 2048 x 5632: 8.3 -> 7.9), except where that leaves NT = 128 four
+  // stages instead of six (128 x 4096 x 14336: 19.0 -> 19.3).
+  static constexpr bool kBeside = NT < 128;
+  static constexpr int beside_bytes(bool split) { return kBeside && split ? kPartBytes : 0; }
   // The ring that leaves room for `ctas` CTAs on an SM, and for no more of them than tensor memory serves.
-  static constexpr int stages_for(int ctas) {
-    const int n = (kSmemPerSm / ctas - kSmemReserved - kExtraBytes) / kStageBytes;
+  static constexpr int stages_for(int ctas, bool split) {
+    const int n = (kSmemPerSm / ctas - kSmemReserved - kExtraBytes - beside_bytes(split)) / kStageBytes;
     return n < kMaxStages ? n : kMaxStages;
   }
   // Two threads may issue if neither can test a stage's barrier a phase early.  A thread that turns to block i has found
   // block i - 2 open, so the blocks up to i - 2 - kBufs are done; the stage's block before, i - stages, is among them, or
   // is the same thread's (stages even).
   static constexpr int issue_step(int stages) { return stages % 2 == 0 || stages >= kBufs + 2 ? 2 : 1; }
-  static constexpr int smem_bytes(int stages) { return stages * kStageBytes + kExtraBytes; }
-  static_assert((kTokenRows ? 1 : 2) * NT * kPartFloats * 4 <= 3 * kStageBytes, "the parts overlay the ring");
-  static_assert(stages_for(kCtasPerSm) >= kBufs && stages_for(kCtasPerSm) >= 3, "a stage comes round no sooner than a buffer");
+  static constexpr int smem_bytes(int stages, bool split) {
+    return stages * kStageBytes + kExtraBytes + beside_bytes(split);
+  }
+  static constexpr int kMinStages = kBufs > 3 ? kBufs : 3;
+  static_assert(NT * kPartFloats * 4 <= kMinStages * kStageBytes, "the parts overlay the ring");
+  static_assert(stages_for(kCtasPerSm, false) >= kMinStages, "a stage comes round no sooner than a buffer");
+  static_assert(kMoveRegs || stages_for(1, true) >= kMinStages, "a cluster's CTAs");
   static_assert(kCtasPerSm * kTmemCols <= 512, "tensor memory");
 };
 
@@ -174,7 +184,8 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
   uint8_t* smem_w = smem;
   uint8_t* smem_x = smem + stages * Cfg::kWeightBytes;
   float* scales = reinterpret_cast<float*>(smem + stages * Cfg::kStageBytes);  // [kScaleBlocks][NT]
-  float* parts = reinterpret_cast<float*>(smem);  // after the main loop: [S][NT / S][kPartFloats], this CTA's tokens
+  // [S][NT / S][kPartFloats], this CTA's tokens; over the ring, or beside it
+  float* parts = reinterpret_cast<float*>(Cfg::kBeside && S > 1 ? smem + stages * Cfg::kStageBytes + Cfg::kExtraBytes : smem);
   uint64_t* full = reinterpret_cast<uint64_t*>(scales + Cfg::kScaleBlocks * NT);  // [stages]
   uint64_t* done = full + Cfg::kMaxStages;                                     // [stages]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + Cfg::kMaxStages);
@@ -202,6 +213,7 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
+  if (Cfg::kBeside && S > 1) cluster_arrive();  // waited for before the first push: the cluster's CTAs are all there
   pdl_trigger();  // tensor memory is allocated: the next kernel may be scheduled
   // The first weight tiles are asked into L2 while the previous kernel ends (nothing in flight writes weights, and L2 is
   // the point of coherence); everything that reads or writes global memory for good waits for it.
@@ -334,10 +346,11 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
     }
     tc_fence_before_sync();
     __syncwarp();
-    if (S > 1)
-      cluster_sync_all();  // the rings of the whole cluster are free
-    else
-      promote_sync<128 * Cfg::kGroups>();
+    if (S > 1) {
+      if (!Cfg::kBeside) cluster_arrive();  // the rings of the whole cluster are free
+      cluster_wait();
+    }
+    if (S == 1 || !Cfg::kTokenRows) promote_sync<128 * Cfg::kGroups>();
     if (ok && Cfg::kTokenRows && row < tokens) {
       const uint32_t mine = smem_u32(parts) + (uint32_t)((rank * per + row % per) * Cfg::kPartFloats + col0) * 4u;
       const uint32_t at = S > 1 ? dsmem_addr(mine, (uint32_t)(row / per)) : mine;
@@ -377,7 +390,8 @@ gemm_blocks_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gr
   }
   if (warp >= kPromoteWarps && S > 1) {  // the two barriers of the cluster above (barriers are all that may follow here:
     __syncwarp();                        // with NT = 128 these warps are down to 32 registers)
-    cluster_sync_all();
+    if (!Cfg::kBeside) cluster_arrive();
+    cluster_wait();
     cluster_sync_all();
   }
   __syncthreads();
@@ -405,12 +419,12 @@ static int launch_decode_as(const Ctx* ctx, cudaStream_t stream, const GemmBlock
   CUtensorMap tw, tx;
   if (int rc = make_tmap_2d(ctx, &tw, p.b, 1, (uint64_t)p.K, (uint64_t)p.N, (uint64_t)p.ldb, kBKBytes, kBM)) return rc;
   if (int rc = make_tmap_2d(ctx, &tx, p.a, 1, (uint64_t)p.K, (uint64_t)p.M, (uint64_t)p.lda, kBKBytes, NT)) return rc;
-  if (int rc = ensure_dynamic_smem<gemm_blocks_decode_kernel<NT, kAlone>>(ctx, Cfg::smem_bytes(Cfg::stages_for(1)),
+  if (int rc = ensure_dynamic_smem<gemm_blocks_decode_kernel<NT, kAlone>>(ctx, Cfg::kSmemPerSm - Cfg::kSmemReserved,
                                                                           "gemm_blocks_decode_kernel"))
     return rc;
-  const int stages = Cfg::stages_for(per_sm < Cfg::kCtasPerSm ? per_sm : Cfg::kCtasPerSm);
+  const int stages = Cfg::stages_for(per_sm < Cfg::kCtasPerSm ? per_sm : Cfg::kCtasPerSm, S > 1);
   cudaError_t e = launch_kernel(gemm_blocks_decode_kernel<NT, kAlone>, dim3((unsigned)(tiles_n * S), (unsigned)tiles_m),
-                                dim3(Cfg::kThreads), Cfg::smem_bytes(stages), stream, (unsigned)S, tw, tx, p, S, stages);
+                                dim3(Cfg::kThreads), Cfg::smem_bytes(stages, S > 1), stream, (unsigned)S, tw, tx, p, S, stages);
   if (e != cudaSuccess) {
     set_last_error("gemm_blocks_decode_kernel launch: %s", cudaGetErrorString(e));
     return XAXB_LAUNCH_FAILED;
