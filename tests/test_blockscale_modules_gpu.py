@@ -269,3 +269,26 @@ def test_first_call_captured():
     graph.replay()
     assert same(eager, want) and same(got, want)
     assert same(got_own, eager_own)
+
+
+def test_transformer_on_block_scaled_layers():
+    """The token-in, logits-out module: batched self-attention casts its input once, sequence by sequence alike, and a token
+    does not depend on those behind it (every scale belongs to one token)."""
+    from xax_b200 import Transformer, apply_linear, ops
+
+    model = Transformer.build(64, 256, 4, 512, 2, 64, key=1, causal=True, use_rotary_embeddings=True, use_fp8=True, fp8_blocks=True)
+    assert all(b.self_attn.is_fp8_blocks() and b.feed_forward.is_fp8_blocks() for b in model.layers.layers)
+    attn = model.layers.layers[0].self_attn
+    assert not attn.use_fp8
+    x = randn(2, 9, 256, seed=3)
+    out = attn(x)
+    assert out.shape == x.shape and same(out[1], attn(x[1:])[0])
+    assert same(attn.q_proj.forward_quantized(*ops.quantize_blocks(x.reshape(18, 256))),
+                apply_linear(x, attn.q_proj).reshape(18, 256))
+    tokens = torch.arange(16, device="cuda", dtype=torch.int32)
+    logits, _ = model.forward(tokens)
+    assert logits.shape == (16, 64) and torch.isfinite(logits).all()
+    hidden, x = model.encode(tokens)[0], model.token_embedding(tokens[0]).reshape(1, 256)
+    for block in model.layers.layers:  # the first token, alone through the blocks
+        x, _ = block.forward(x)
+    assert rel(model.layer_norm(x), hidden[:1]) < 2.0**-6  # (a few bf16 and e4m3 roundings may fall the other way)

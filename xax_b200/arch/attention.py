@@ -409,7 +409,7 @@ class SelfAttentionBlock:
         return cls(mk(embed_dim, qd, seed + 1), mk(embed_dim, kd, seed + 2), mk(embed_dim, kd, seed + 3),
                    mk(qd, embed_dim, seed + 4), rope, qn, kn, sinks, num_heads=num_heads, num_kv_heads=kv, head_dim=hd,
                    causal=causal, local_window_size=None if context_length is None else context_length - 1,  # :660
-                   use_fp8=use_fp8).stack_weights()
+                   use_fp8=use_fp8 and not fp8_blocks).stack_weights()
 
     def stack_weights(self) -> "SelfAttentionBlock":
         """Block-scaled q, k and v layers that this library has just made share one operand."""
@@ -533,6 +533,9 @@ class SelfAttentionBlock:
         projs = (self.q_proj, self.k_proj, self.v_proj)
         if self._is_fp8():  # the three layers quantise the same tensor the same way: do it once
             xq, _, x_inv, _ = ops.quantize_current(x2, B * T)
+            q, k, v = (p.forward_quantized(xq, x_inv) for p in projs)
+        elif self.is_fp8_blocks():
+            xq, x_inv = ops.quantize_blocks(x2)
             q, k, v = (p.forward_quantized(xq, x_inv) for p in projs)
         else:
             q, k, v = (apply_linear(x2, p) for p in projs)
@@ -941,7 +944,8 @@ class TransformerStack:
               cross_attention: bool = False, context_length: int | None = None, use_rotary_embeddings: bool = False,
               rotary_base: float = 10000.0, use_fp8: bool = False, compute_dtype=BF16, norm_type: str = "rmsnorm",
               feedforward_type: str = "swiglu", num_kv_heads: int | None = None, head_dim: int | None = None,
-              norm_eps: float = 1e-6, fp8_mlp: bool | None = None, device=None) -> "TransformerStack":
+              norm_eps: float = 1e-6, fp8_mlp: bool | None = None, device=None,
+              fp8_blocks: bool = False) -> "TransformerStack":
         seed = int(key or 0) if not isinstance(key, torch.Generator) else int(key.initial_seed())
         layers = tuple(
             TransformerBlock.build(embed_dim, num_heads, ff_dim, key=seed * 1000 + i, num_kv_heads=num_kv_heads,
@@ -949,7 +953,7 @@ class TransformerStack:
                                    context_length=context_length, use_rotary_embeddings=use_rotary_embeddings,
                                    rotary_base=rotary_base, norm_type=norm_type, norm_eps=norm_eps,
                                    feedforward_type=feedforward_type, use_fp8=use_fp8, compute_dtype=compute_dtype,
-                                   fp8_mlp=fp8_mlp, device=device)
+                                   fp8_mlp=fp8_mlp, device=device, fp8_blocks=fp8_blocks)
             for i in range(num_layers))
         return cls(layers, num_layers, causal, use_fp8)
 

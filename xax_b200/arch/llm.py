@@ -143,7 +143,7 @@ class LLM:
                 if config.use_attention_sinks else None,
                 local_window_size=layer_window,  # context_length = window + 1 (:131), local_window_size = that - 1 (:660)
                 num_heads=config.q_heads // tp_size, num_kv_heads=config.kv_heads // tp_size, head_dim=D, causal=True,
-                use_fp8=use_fp8).stack_weights()
+                use_fp8=use_fp8 and not fp8_blocks).stack_weights()
             mlp = SwiGLU(lin(width, H, "gate_proj", config.mlp_bias), lin(width, H, "up_proj", config.mlp_bias),
                          lin(H, width, "down_proj", config.mlp_bias)).stack_weights()
             blocks.append(TransformerBlock(attn, mlp, RMSNorm.build(H, config.rms_eps, dev),
