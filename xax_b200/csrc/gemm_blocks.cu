@@ -453,10 +453,11 @@ static int launch_decode(const Ctx* ctx, cudaStream_t stream, const GemmBlocksPa
 // promotion could hide behind the MMAs; what bounds the kernel is the turnaround of a buffer: 350 cycles from its
 // release until the issuing thread sees it, 512 of MMAs, 400 from the commit until the promoting warps see that, 330 until
 // they have read it, shared by two buffers: about 900 a block, 62 % of the tensor pipe (without readout and promotion
-// 341 us of 433, and no less with a quarter of the MMAs).  4096 x 28672 x 4096: 421 us = 2.28 PFLOP/s in a graph, 480
-// under the power cap; 2048 x 8192 x 2048: 37.2.  Not faster: 128 x 256 tiles on single CTAs, whose releases are local but
+// 341 us of 433, and no less with a quarter of the MMAs).  4096 x 28672 x 4096: 421 us = 2.28 PFLOP/s in a graph, 480 for
+// seconds on end at the power cap (1455 MHz; the product without block scales: 385 at 1255 MHz); 2048 x 8192 x 2048: 37.2.  Not faster: 128 x 256 tiles on single CTAs, whose releases are local but
 // which read half as much again out of L2 (467 against 419 us); halves of 128 columns with barriers of their own (578);
-// opening the next block before the last columns of this one are added (490).  To keep the turnaround short
+// opening the next block before the last columns of this one are added (490); tiles of 160
+// columns with three buffers (573 against 414).  To keep the turnaround short
 //   * two warps issue, one the even and one the odd K blocks (different buffers, nothing to order between them);
 //   * one barrier opens a K block: full[s] counts both CTAs' copies AND the 16 warps that free the buffer, the latter
 //     arriving on the stage that the block two further on will use;
