@@ -450,14 +450,15 @@ static int launch_decode(const Ctx* ctx, cudaStream_t stream, const GemmBlocksPa
 // core fills the other buffer.
 //
 // Per 128-byte K block the tensor core needs 512 cycles and the packed multiply-adds of two warps per scheduler 256, so the
-// promotion could hide behind the MMAs; what bounds the kernel is the turnaround of a buffer: 350 cycles from its
-// release until the issuing thread sees it, 512 of MMAs, 400 from the commit until the promoting warps see that, 330 until
-// they have read it, shared by two buffers: about 900 a block, 62 % of the tensor pipe (without readout and promotion
-// 341 us of 433, and no less with a quarter of the MMAs).  4096 x 28672 x 4096: 421 us = 2.28 PFLOP/s in a graph, 480 for
-// seconds on end at the power cap (1455 MHz; the product without block scales: 385 at 1255 MHz); 2048 x 8192 x 2048: 37.2.  Not faster: 128 x 256 tiles on single CTAs, whose releases are local but
-// which read half as much again out of L2 (467 against 419 us); halves of 128 columns with barriers of their own (578);
-// opening the next block before the last columns of this one are added (490); tiles of 160
-// columns with three buffers (573 against 414).  To keep the turnaround short
+// promotion could hide behind the MMAs, but a block takes about 900 (62 % of the tensor pipe).  It is a chain of signals: 350
+// cycles from a buffer's release until the issuing thread sees it, 512 of MMAs, 400 from the commit until the promoting
+// warps see that, 330 until they have read it, shared by two buffers.  (Without readout and promotion 341 us of 433, and no
+// less with a quarter of the MMAs; but three buffers of 160 columns do not help, 573 us, or 510 without readout and promotion:
+// a block costs about the same however narrow.)  4096 x 28672 x 4096: 405 to 450 us from GPU to GPU in a graph = 2.1 to 2.4
+// PFLOP/s; for seconds on end 480 us, 1455 MHz at the power cap, where the product without block scales takes 385 at 1255
+// MHz.  2048 x 8192 x 2048: 37 to 43.  Not faster: 128 x 256 tiles on single CTAs, whose releases are local but which read
+// half as much again out of L2 (467 against 419 us); halves of 128 columns with barriers of their own (578); opening the
+// next block before the last columns of this one are added (490).  To keep the chain short
 //   * two warps issue, one the even and one the odd K blocks (different buffers, nothing to order between them);
 //   * one barrier opens a K block: full[s] counts both CTAs' copies AND the 16 warps that free the buffer, the latter
 //     arriving on the stage that the block two further on will use;
