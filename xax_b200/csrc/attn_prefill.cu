@@ -77,8 +77,11 @@ constexpr int kPfThreads = 192;  // warps 0-3: one query row per thread; warp 4:
 //   bar_s[2]             S buffer j & 1 holds Q K_j^T (MMA commit); also: K slot j & 1 may be reloaded
 //   bar_p                the probabilities of tile j are in shared memory, fenced (4 arrivals); also: the
 //                        softmax warps have read S buffer j & 1 out of tensor memory
-//   bar_o                P_j V_j has been added to the accumulator (MMA commit); also: V slot j & 1 and the
-//                        P buffer may be rewritten
+//   bar_o[2]             P_j V_j has been added to the accumulator (MMA commit on bar_o[j & 1]); also: V slot j & 1 and
+//                        the P buffer may be rewritten.  (One for each slot: with a single barrier two phases, P_{j-1} V_{j-1}
+//                        and P_j V_j, could complete before the loader came to test for the first, and a parity cannot tell
+//                        that from none.  P_{j+1} V_{j+1}, the next on the same slot's, needs the V that the loader brings
+//                        after its test.)
 // (j counts the key tiles a CTA has walked since it started, over all its work items.)
 //
 // Work distribution.  A work item is one 128-query tile of one head of one sequence.  Under the causal mask
@@ -106,8 +109,8 @@ __global__ void __launch_bounds__(kPfThreads, 2) attn_prefill_kernel(const __gri
   uint64_t* bar_v = bars + 2;      // [2]
   uint64_t* bar_s = bars + 4;      // [2]
   uint64_t* bar_p = bars + 6;
-  uint64_t* bar_o = bars + 7;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 8);
+  uint64_t* bar_o = bars + 7;      // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 9);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -116,6 +119,7 @@ __global__ void __launch_bounds__(kPfThreads, 2) attn_prefill_kernel(const __gri
     for (int i = 0; i < 6; ++i) mbar_init(bars + i, 1);
     mbar_init(bar_p, 4);
     mbar_init(bar_o, 1);
+    mbar_init(bar_o + 1, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -212,7 +216,7 @@ __global__ void __launch_bounds__(kPfThreads, 2) attn_prefill_kernel(const __gri
         const int g = gb + j;
         // the V slot of tile j + 1 was last read by P V of tile j - 1
         if (j >= 1 && j + 1 < n_tiles) {
-          ok = mbar_wait(bar_o, (g - 1) & 1, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSitePfO);
+          ok = mbar_wait(bar_o + ((g - 1) & 1), ((g - 1) >> 1) & 1, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSitePfO);
           if (!ok) break;
           load_v(j + 1);
         }
@@ -265,7 +269,7 @@ __global__ void __launch_bounds__(kPfThreads, 2) attn_prefill_kernel(const __gri
           umma_f16(tmem_pv, umma_desc_kmajor_sw128(smem_u32(sP) + k * 32),
                    umma_desc_mnmajor_sw128(smem_u32(v_src) + k * 16 * 128, SM::kKVHalfBytes), idesc, (j | k) != 0);
         }
-        umma_commit(bar_o);
+        umma_commit(bar_o + (g & 1));
       }
     }
   } else {
@@ -352,7 +356,7 @@ __global__ void __launch_bounds__(kPfThreads, 2) attn_prefill_kernel(const __gri
       // ---- the previous tile's P V must be complete before its P operand or the accumulator are touched;
       // by now it usually is (the exponentials above ran under it)
       if (j > 0) {
-        ok = ok && mbar_wait(bar_o, (g - 1) & 1, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSitePfO);
+        ok = ok && mbar_wait(bar_o + ((g - 1) & 1), ((g - 1) >> 1) & 1, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSitePfO);
         if (ok) tc_fence_after_sync();
       }
       // ---- lazy rescale of the row's accumulator ------------------------------------------------
@@ -391,7 +395,8 @@ __global__ void __launch_bounds__(kPfThreads, 2) attn_prefill_kernel(const __gri
       if (lane == 0) mbar_arrive(bar_p);  // the issuer queues O += P V behind this
     }
     if (ok) {
-      ok = mbar_wait(bar_o, (gb + n_tiles - 1) & 1, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSitePfO);
+      const int g = gb + n_tiles - 1;
+      ok = mbar_wait(bar_o + (g & 1), (g >> 1) & 1, abort_flag, p.d_status, XAXB_DEVICE_TIMEOUT * 1000 + kSitePfO);
       if (ok) tc_fence_after_sync();
     }
     __syncwarp();
