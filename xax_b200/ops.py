@@ -254,10 +254,13 @@ def _check_rows(what: str, t: torch.Tensor, dtype, name: str, shape=None) -> Non
         raise ValueError(f"{what}: {name} must be {list(shape)}, got {tuple(t.shape)}")
 
 
+_current_device = torch._C._cuda_getDevice  # (torch.cuda.current_device without its test for a started CUDA)
+
+
 def _device_of(t: torch.Tensor) -> int:
     """The current device if ``t`` is on it, else -2 (on which no tensor is, so that the helpers get to refuse it)."""
     device = t.get_device()  # -1 for a CPU tensor
-    return device if device >= 0 and device == torch.cuda.current_device() else -2
+    return device if device >= 0 and device == _current_device() else -2
 
 
 def quantize_blocks(x: torch.Tensor, block_rows: int = 1):
@@ -287,17 +290,21 @@ def gemm_fp8_blocks(a_q, b_q, a_inv, b_inv, bias=None, residual=None, out=None):
     a multiple of 16 and N of 8.  ``out`` may be ``residual``; otherwise it must not overlap an operand."""
     what = "gemm_fp8_blocks"
     dev = _device_of(a_q)
-    if not (_is_input(a_q, E4M3, 2, dev) and _is_input(b_q, E4M3, 2, dev)):  # (contiguous, or rows apart: both will do)
+    whole = (a_q.dtype is E4M3 and b_q.dtype is E4M3 and a_q.is_contiguous() and b_q.is_contiguous()
+             and b_q.get_device() == dev and a_q.dim() == 2 and b_q.dim() == 2)
+    if not whole:  # (contiguous, or rows apart: both will do)
         _check_rows(what, a_q, E4M3, "a_q")
         _check_rows(what, b_q, E4M3, "b_q")
         dev = a_q.get_device()
     (M, K), (N, Kb) = a_q.shape, b_q.shape
+    lda, ldb = (K, K) if whole else (a_q.stride(0) if M > 1 else K, b_q.stride(0))  # (a single row's stride may be anything)
     if K != Kb:
         raise ValueError(f"{what}: inner dimensions differ ({K} vs {Kb})")
-    if not (_is_input(a_inv, F32, 2, dev) and _is_input(b_inv, F32, 2, dev)):
+    if not (a_inv.dtype is F32 and b_inv.dtype is F32 and a_inv.is_contiguous() and b_inv.is_contiguous()
+            and a_inv.get_device() == dev and b_inv.get_device() == dev):
         a_inv, b_inv = _block_input(what, a_inv, F32, "a_inv"), _block_input(what, b_inv, F32, "b_inv")
     blocks = -(-K // SCALE_BLOCK)
-    if a_inv.shape != (M, blocks) or b_inv.shape != (-(-N // SCALE_BLOCK), blocks):
+    if a_inv.shape != (M, blocks) or b_inv.shape != (-(-N // SCALE_BLOCK), blocks):  # (their rank, too)
         raise ValueError(f"{what}: a_inv {tuple(a_inv.shape)} and b_inv {tuple(b_inv.shape)} must be "
                          f"({M}, {blocks}) and ({_blocks(N)}, {blocks})")
     bias_ptr = res_ptr = None
@@ -309,19 +316,21 @@ def gemm_fp8_blocks(a_q, b_q, a_inv, b_inv, bias=None, residual=None, out=None):
             raise ValueError(f"{what}: bias must be [{N}], got {tuple(bias.shape)}")
         bias_ptr = bias.data_ptr()
     if residual is not None:
+        res_ptr, ldr = residual.data_ptr(), N
         if residual.shape != (M, N) or not _is_input(residual, BF16, 2, dev):
             _check_rows(what, residual, BF16, "residual", (M, N))
-        res_ptr, ldr = residual.data_ptr(), residual.stride(0) if M > 1 else N
+            ldr = residual.stride(0) if M > 1 else N
+    ldo = N
     if out is None:
         out = a_q.new_empty(M, N, dtype=BF16)
     else:
         _check_rows(what, out, BF16, "out", (M, N))
+        ldo = out.stride(0) if M > 1 else N
     if M == 0:
         return out
-    lda, ldo = (a_q.stride(0), out.stride(0)) if M > 1 else (K, N)  # the stride of a single row may be anything
     ctx, st, lib = _lib.call_state(dev)
-    check(lib.xaxb_gemm_fp8_blocks(ctx, st, a_q.data_ptr(), lda, a_inv.data_ptr(), b_q.data_ptr(), b_q.stride(0),
-                                   b_inv.data_ptr(), M, N, K, bias_ptr, res_ptr, ldr, out.data_ptr(), ldo), what)
+    check(lib.xaxb_gemm_fp8_blocks(ctx, st, a_q.data_ptr(), lda, a_inv.data_ptr(), b_q.data_ptr(), ldb, b_inv.data_ptr(), M,
+                                   N, K, bias_ptr, res_ptr, ldr, out.data_ptr(), ldo), what)
     return out
 
 
